@@ -129,7 +129,7 @@ int lcn_memcpy_d2h(void* handle, void* dst, const void* src, int64_t bytes);
  * (inference.py:70-110, tools/data.py:10-54, 205-322).  These entry points keep
  * the arrays in HBM (in the caller's dtype; float64 is cast to float32 on the
  * device exactly as a float32 feed would) and build every batch there. */
-enum { LCN_DTYPE_F32 = 0, LCN_DTYPE_F64 = 1 };
+enum { LCN_DTYPE_F32 = 0, LCN_DTYPE_F64 = 1, LCN_DTYPE_BF16 = 2, LCN_DTYPE_F16 = 3 };
 enum { LCN_MAX_DATASETS = 16, LCN_MAX_COPIES = 8 };
 /* augmentation op per copy of the virtually concatenated dataset */
 enum {
@@ -238,6 +238,65 @@ int lcn_eval_mpjpe(int32_t device, int64_t n, const double* pred, const double* 
 int lcn_eval_mpjpe_static(int32_t device, int64_t n, const double* pred, const double* gt,
                           const double* box, const double* cam, const double* root_depth,
                           int32_t protocol2, double* err);
+
+/* --- weight and int8 operators (handle-free) ------------------------------- */
+/* These take device memory of the caller's and run on the caller's stream
+ * (hipStream_t; NULL = the device's default stream) of `device`; the calling
+ * thread's current device is unchanged.  They allocate nothing, do not
+ * synchronise and may be captured into a graph.  Scratch memory is the
+ * caller's: `workspace`, 256-byte aligned, at least as many bytes as the
+ * matching _workspace function returns (negative: LCN_E_*); a workspace
+ * belongs to one call at a time in stream order, so calls on two streams (or
+ * two graphs that may run at once) need two.  dtype: LCN_DTYPE_F32, _BF16 or
+ * _F16.  Matrices have a contiguous last dimension; strides are in elements
+ * and not negative; batch strides are unused with batch 1, row strides with one
+ * row.  Operands that would overlap where they must not are LCN_E_ARG, an
+ * empty batch is LCN_OK.  Errors: lcn_last_error(NULL).  No counterpart in the
+ * reference (its optimiser is Adam, models_att.py:404-409; it predicts in
+ * float32, :79-132). */
+
+/* out = NS(in) for batch matrices of rows x cols, Newton-Schulz products:
+ *   X = G / max(|G|_F, eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X
+ * (on the transpose where rows > cols), (a, b, c) = coefficients[0..2].
+ * Muon's are 3.4445, -4.775, 2.0315 with 5 steps.  Products are accurate to
+ * float32 for every dtype.  The polynomial must keep the singular values of X
+ * below 4 and its factor b A + c A A below 64 (beyond: infinities).  A matrix
+ * that holds an infinity or a NaN gives NaN.  out may be `in` itself. */
+int64_t lcn_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
+int lcn_orthogonalize(int32_t device, void* stream, int32_t dtype, int64_t batch, int64_t rows, int64_t cols,
+                      const void* in, int64_t in_batch, int64_t in_row, void* out, int64_t out_batch,
+                      int64_t out_row, int32_t steps, const float* coefficients, float eps, void* workspace,
+                      int64_t workspace_bytes);
+
+/* One Muon step on batch float32 matrices, in place:
+ *   momentum <- beta momentum + grad;  u = grad + beta momentum (nesterov != 0) or momentum
+ *   param <- (1 - lr weight_decay) param - lr scale NS(u)
+ * lr_dev (device memory, one float) is read instead of lr when not NULL, so a
+ * captured graph follows a schedule.  Workspace: lcn_orthogonalize_workspace. */
+int lcn_muon_update(int32_t device, void* stream, int32_t grad_dtype, int64_t batch, int64_t rows, int64_t cols,
+                    float* param, int64_t param_batch, int64_t param_row, float* momentum, int64_t momentum_batch,
+                    int64_t momentum_row, const void* grad, int64_t grad_batch, int64_t grad_row, float lr,
+                    const float* lr_dev, float scale, float beta, int32_t nesterov, float weight_decay,
+                    int32_t steps, const float* coefficients, float eps, void* workspace,
+                    int64_t workspace_bytes);
+
+/* Product in 8-bit integers with one scale a token and one a channel:
+ *   s[t] = max_k |x[t,k]| / 127,  q[t,k] = rint(x[t,k] * (127 / max_k |x[t,k]|))
+ *   out[t,c] = (sum_k q[t,k] weight[c,k]) * s[t] * weight_scale[c] (+ bias[c])
+ * x [tokens][k] and out [tokens][n] of type dtype, weight [n][k] int8, scales
+ * and bias float32.  A row of x whose largest magnitude is below 2^-100 counts
+ * as zero; one that holds an infinity or a NaN gives NaN.  k <= 131072. */
+int64_t lcn_int8_linear_workspace(int64_t tokens, int64_t k, int64_t n);
+int lcn_int8_linear(int32_t device, void* stream, int32_t dtype, int64_t tokens, int64_t k, int64_t n,
+                    const void* x, int64_t x_row, const int8_t* weight, int64_t weight_row,
+                    const float* weight_scale, const float* bias, void* out, int64_t out_row, void* workspace,
+                    int64_t workspace_bytes);
+/* the weights of lcn_int8_linear, once: element (c, k) of w at c stride_n + k
+ * stride_k (so both [n][k] and [k][n] weights); scale[c] = max_k |w| / 127,
+ * q [n][k] = rint(w * (127 / max_k |w|)).  A channel that holds an infinity or
+ * a NaN gets scale NaN and zeros. */
+int lcn_int8_quantize_weight(int32_t device, void* stream, int32_t dtype, int64_t n, int64_t k, const void* w,
+                             int64_t stride_n, int64_t stride_k, int8_t* q, float* scale);
 
 /* --- checkpoint I/O helpers (host only) -------------------------------- */
 /* CRC-32C of TensorFlow tensor-bundle checkpoints (tf.train.Saver files the

@@ -1,0 +1,411 @@
+// Newton-Schulz orthogonalisation of a batch of matrices and the Muon update
+// built on it (gfx950).
+//
+//   X0 = G / max(|G|_F, eps);  steps times:  A = X X^T,  B = b A + c A A,
+//   X <- a X + B X                            (on G^T where rows > cols)
+//
+// The quintic pushes every singular value of X towards 1 (Muon: K. Jordan,
+// 2024; Newton-Schulz iterations: Bjorck & Bowie, 1971).  Muon's update:
+//   buf <- beta buf + g,  u = g + beta buf (Nesterov) or buf,
+//   W <- (1 - lr decay) W - lr scale NS(u).
+//
+// Precision.  The iteration amplifies a perturbation of a small singular
+// direction by up to a^steps (485 for the default): with X in one fp16 the
+// result of a rank-64 gradient is 11 bf16 roundings off.  Every matrix is
+// therefore held as two fp16 numbers, v S = hi + lo / 2048 (22 significant
+// bits), and every product is three fp16 MFMA products, hi hi + (hi lo + lo hi)
+// / 2048, summed in two fp32 accumulators; the dropped lo lo term is below
+// 2^-22 of the result.  Three products at the fp16 rate are still five times
+// the rate of the fp32 MFMA.  S is a power of two per matrix kind that keeps
+// the entries inside fp16's range (|X|, |B| <= 64, |A| <= 16).
+//
+// Layout.  A plane (the hi or the lo half of a matrix with R rows and
+// contraction length K, both padded to 32 with zeros) is stored as
+// [R/32][K/8][32][8] halves: two neighbouring octet columns (32 rows x 16 k) are
+// one 1 KB operand fragment of v_mfma_f32_32x32x16_f16, so global -> LDS copies
+// and LDS -> register reads are linear.  X is kept in both orientations: Xr
+// (rows m, contraction n) for A = X X^T and Xc (rows n, contraction m) for
+// B X; an accumulator holds four consecutive i of one j, which is a contiguous
+// 8-byte piece of the (row j, contraction i) form, and the other form is
+// transposed through LDS.
+#include <algorithm>
+
+#include "ops_common.h"
+
+namespace lcn {
+
+namespace {
+
+constexpr float kSx = 1024.f, kSa = 4096.f, kSb = 1024.f;  // scales of X, A, B
+constexpr float kLo = 2048.f;                              // scale of the lo halves
+constexpr int kNormParts = 64;                             // partial sums of squares per matrix
+
+__host__ __device__ inline int64_t pad32(int64_t v) { return (v + 31) / 32 * 32; }
+
+// per-matrix workspace, in bytes from its start
+struct NsPlan {
+  int m, n;                 // short / long side
+  int mp, np;               // padded
+  int64_t xplane, aplane;   // bytes of a plane
+  int64_t x[2], a, b;       // Xr hi, Xr lo, Xc hi, Xc lo (twice); A hi, lo; B hi, lo
+  int64_t stride;
+};
+NsPlan make_plan(int64_t rows, int64_t cols) {
+  NsPlan p;
+  p.m = (int)std::min(rows, cols);
+  p.n = (int)std::max(rows, cols);
+  p.mp = (int)pad32(p.m);
+  p.np = (int)pad32(p.n);
+  p.xplane = (int64_t)p.mp * p.np * 2;
+  p.aplane = (int64_t)p.mp * p.mp * 2;
+  p.x[0] = 0;
+  p.x[1] = 4 * p.xplane;
+  p.a = 8 * p.xplane;
+  p.b = p.a + 2 * p.aplane;
+  p.stride = p.b + 2 * p.aplane;
+  return p;
+}
+
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  lo = (_Float16)((v - (float)hi) * kLo);
+}
+
+// ---- norm (and, for muon, the momentum update) ---------------------------------------------
+// part[b][p] = sum of squares, in float64, of the rows this workgroup walks.
+template <int T, bool kMuon>
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restrict__ part) {
+  __shared__ double red[4];
+  const int64_t b = blockIdx.y;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  double s = 0.0;
+  for (int r = blockIdx.x * 4 + ty; r < a.rows; r += gridDim.x * 4) {
+    const int64_t g0 = b * a.in.batch + (int64_t)r * a.in.row;
+    float* mom = kMuon ? (float*)a.momentum.p + b * a.momentum.batch + (int64_t)r * a.momentum.row : nullptr;
+    for (int c = tx; c < a.cols; c += 64) {
+      float v = op_load<T>(a.in.p, g0 + c);
+      if constexpr (kMuon) {
+        const float m = fmaf(a.beta, mom[c], v);
+        mom[c] = m;
+        v = a.nesterov ? fmaf(a.beta, m, v) : m;
+      }
+      s += (double)v * (double)v;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (tx == 0) red[ty] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[b * kNormParts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ---- X0 in both orientations ---------------------------------------------------------------
+template <int T, bool kMuon>
+__global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, NsPlan p, int parts, const double* __restrict__ part,
+                                                      char* __restrict__ ws) {
+  __shared__ unsigned tile[32 * 33];
+  const int64_t b = blockIdx.y;
+  const int nb = p.np / 32;
+  const int bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;  // 32-row block of X, 32-column block
+  const int lane = threadIdx.x & 63;
+  double s = lane < parts ? part[b * kNormParts + lane] : 0.0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  const double inv = (double)kSx / fmax(sqrt(s), (double)a.eps);
+  const bool bad = !(s < 1e300);  // an infinity or a NaN in the matrix: every entry becomes NaN
+  const bool tall = a.rows > a.cols;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    // fast index tx along the source's rows; (i, j) of X
+    const int sr = ty + 8 * q;
+    const int i = tall ? tx : sr, j = tall ? sr : tx;
+    const int gi = bi * 32 + i, gj = bj * 32 + j;
+    float v = 0.f;
+    if (gi < p.m && gj < p.n) {
+      const int64_t r = tall ? gj : gi, c = tall ? gi : gj;
+      v = op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c);
+      if constexpr (kMuon) {
+        const float m = ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c];
+        v = a.nesterov ? fmaf(a.beta, m, v) : m;
+      }
+      v = bad ? __builtin_nanf("") : (float)((double)v * inv);
+    }
+    _Float16 hi, lo;
+    split(v, hi, lo);
+    tile[i * 33 + j] = (unsigned)__builtin_bit_cast(unsigned short, hi) | ((unsigned)__builtin_bit_cast(unsigned short, lo) << 16);
+  }
+  __syncthreads();
+  // 32 x 4 octets in either form: threads 0..127 Xr (row i, contraction j), 128..255 Xc
+  const int t = threadIdx.x & 127, row = t & 31, u = t >> 5;
+  const bool xc = threadIdx.x >= 128;
+  unsigned short hs[8], ls[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const unsigned w = xc ? tile[(8 * u + e) * 33 + row] : tile[row * 33 + 8 * u + e];
+    hs[e] = (unsigned short)w;
+    ls[e] = (unsigned short)(w >> 16);
+  }
+  const int64_t unit = xc ? ((int64_t)bj * (p.mp / 8) + bi * 4 + u) * 32 + row : ((int64_t)bi * (p.np / 8) + bj * 4 + u) * 32 + row;
+  char* x = ws + b * p.stride + p.x[0] + (xc ? 2 * p.xplane : 0);
+  *(v4u*)(x + unit * 16) = *(v4u*)hs;
+  *(v4u*)(x + p.xplane + unit * 16) = *(v4u*)ls;
+}
+
+// ---- the three products --------------------------------------------------------------------
+enum { kGram = 0, kSquare = 1, kUpdate = 2, kFinal = 3 };
+
+struct NsProd {
+  const char* P; const char* Q;       // hi planes of matrix 0; lo planes follow at p_lo / q_lo
+  int64_t p_lo, q_lo;
+  int Rp, Rq, K;                      // rows (multiples of 32) of P and Q, contraction length
+  int64_t stride;                     // bytes between the matrices' workspaces
+  int ti, tj;                         // 128-row tiles of P and Q
+  int tiles;                          // tiles of a matrix
+  const char* E; int64_t e_lo;        // kSquare: A (= Q); kUpdate / kFinal: Xc, in (row j, contraction i) form
+  char* Y; int64_t y_lo;              // result in (row j, contraction i) form
+  char* Z; int64_t z_lo;              // result in (row i, contraction j) form
+  float f, e;                         // result = f * sum + e * E  (scales of the stored forms folded in)
+};
+
+#define NS_LDS(SRC, VOFF, SOFF, DST) \
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
+
+// One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 32
+// through a double LDS buffer filled by LDS-DMA (32 KB a stage: hi and lo of
+// both operands).  All fragments of a stage are read before the next stage's
+// loads are issued, so no LDS read waits for them.
+template <int MODE, int T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void ns_prod_kernel(NsProd g, NsArgs a, NsPlan pl) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * 32768];
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mat = id / g.tiles, t = id - mat * g.tiles;
+  int ti, tj;
+  if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle: ti >= tj
+    ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > t) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+    tj = t - ti * (ti + 1) / 2;
+  } else {
+    ti = t % g.ti;
+    tj = t / g.ti;
+  }
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = w >> 1, wj = w & 1, h = lane >> 5, l31 = lane & 31;
+  const char* Pm = g.P + mat * g.stride;
+  const char* Qm = g.Q + mat * g.stride;
+  const int nPb = g.Rp / 32, nQb = g.Rq / 32;
+  // this wave stages row block w of both operand tiles (a block past the end
+  // repeats the last one; its results are not stored)
+  const int rb_bytes = g.K * 64;
+  const int pb = min(ti * 4 + w, nPb - 1), qb = min(tj * 4 + w, nQb - 1);
+  const __amdgpu_buffer_rsrc_t rph = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rpl = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + g.p_lo + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
+  const int vo = lane * 16;
+  // stage layout: P hi | P lo | Q hi | Q lo, 8 KB each = 4 row blocks x 2 KB
+  auto stage = [&](int ks, int buf) {
+    char* d = lds + buf * 32768 + w * 2048;
+    const int so = ks * 2048;
+    NS_LDS(rph, vo, so, d);                NS_LDS(rph, vo, so + 1024, d + 1024);
+    NS_LDS(rpl, vo, so, d + 8192);         NS_LDS(rpl, vo, so + 1024, d + 8192 + 1024);
+    NS_LDS(rqh, vo, so, d + 16384);        NS_LDS(rqh, vo, so + 1024, d + 16384 + 1024);
+    NS_LDS(rql, vo, so, d + 24576);        NS_LDS(rql, vo, so + 1024, d + 24576 + 1024);
+  };
+  f32x16 acc[2][2], cr[2][2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) { acc[x][y][e] = 0.f; cr[x][y][e] = 0.f; }
+  const int nk = g.K / 32;
+  stage(0, 0);
+  __syncthreads();
+  for (int ks = 0; ks < nk; ++ks) {
+    const char* s = lds + (ks & 1) * 32768;
+    half8 ph[2][2], plo[2][2], qh[2][2], qlo[2][2];  // [row block][k16]
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int op = (wi * 2 + x) * 2048 + kk * 1024 + vo, oq = (wj * 2 + x) * 2048 + kk * 1024 + vo;
+        ph[x][kk] = *(const half8*)(s + op);
+        plo[x][kk] = *(const half8*)(s + 8192 + op);
+        qh[x][kk] = *(const half8*)(s + 16384 + oq);
+        qlo[x][kk] = *(const half8*)(s + 24576 + oq);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (ks + 1 < nk) stage(ks + 1, (ks + 1) & 1);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x][kk], qh[y][kk], acc[x][y], 0, 0, 0);
+          cr[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x][kk], qlo[y][kk], cr[x][y], 0, 0, 0);
+          cr[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(plo[x][kk], qh[y][kk], cr[x][y], 0, 0, 0);
+        }
+    __syncthreads();
+  }
+  // epilogue, one 32 x 32 block at a time; the wave transposes in its own 4.2 KB of LDS
+  unsigned* tr = (unsigned*)lds + w * (32 * 33);
+  const float lr = MODE == kFinal && a.momentum.p ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int rbi = ti * 4 + wi * 2 + x, rbj = tj * 4 + wj * 2 + y;
+      if (rbi >= nPb || rbj >= nQb) continue;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = fmaf(cr[x][y][e], 1.f / kLo, acc[x][y][e]) * g.f;
+      // (row j, contraction i): octet 4 rbi + q of row block rbj, row l31, halves 4h .. 4h + 3
+      const int64_t at = (((int64_t)rbj * (g.Rp / 8) + rbi * 4) * 32 + l31) * 16 + h * 8;
+      if constexpr (MODE != kGram) {
+        const char* E = g.E + mat * g.stride + at;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const half4 eh = *(const half4*)(E + q * 512), el = *(const half4*)(E + g.e_lo + q * 512);
+#pragma unroll
+          for (int s2 = 0; s2 < 4; ++s2) v[4 * q + s2] = fmaf(fmaf((float)el[s2], 1.f / kLo, (float)eh[s2]), g.e, v[4 * q + s2]);
+        }
+      }
+      if constexpr (MODE == kFinal) {
+        const bool tall = a.rows > a.cols;
+        const int j = rbj * 32 + l31;
+        if (j < pl.n) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = rbi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+            if (i >= pl.m) continue;
+            const int64_t o = (int64_t)mat * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j);
+            if (a.momentum.p) {
+              float* W = (float*)a.out.p + o;
+              *W = fmaf(-lr * a.scale, v[e], *W * (1.f - lr * a.decay));
+            } else {
+              op_store<T>(a.out.p, o, v[e]);
+            }
+          }
+        }
+      } else {
+        char* Y = g.Y + mat * g.stride + at;
+        unsigned word[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          half4 hv, lv;
+#pragma unroll
+          for (int s2 = 0; s2 < 4; ++s2) {
+            _Float16 hi, lo;
+            split(v[4 * q + s2], hi, lo);
+            hv[s2] = hi;
+            lv[s2] = lo;
+            word[4 * q + s2] = (unsigned)__builtin_bit_cast(unsigned short, hi) | ((unsigned)__builtin_bit_cast(unsigned short, lo) << 16);
+          }
+          *(half4*)(Y + q * 512) = hv;
+          *(half4*)(Y + g.y_lo + q * 512) = lv;
+        }
+        if (MODE == kUpdate || ti != tj) {  // the other form: (row i, contraction j)
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) tr[(8 * (e >> 2) + 4 * h + (e & 3)) * 33 + l31] = word[e];
+          __builtin_amdgcn_wave_barrier();
+          char* Z = g.Z + mat * g.stride + (((int64_t)rbi * (g.Rq / 8) + rbj * 4) * 32 + l31) * 16;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            unsigned short hs[8], ls[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const unsigned wd = tr[l31 * 33 + 8 * (2 * u + h) + e];
+              hs[e] = (unsigned short)wd;
+              ls[e] = (unsigned short)(wd >> 16);
+            }
+            *(v4u*)(Z + (2 * u + h) * 512) = *(v4u*)hs;
+            *(v4u*)(Z + g.z_lo + (2 * u + h) * 512) = *(v4u*)ls;
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+}
+
+template <int MODE, int T>
+void launch_prod(const NsProd& g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((ns_prod_kernel<MODE, T>), dim3((unsigned)(g.tiles * a.batch)), dim3(256), 0, s, g, a, p);
+}
+
+template <int T>
+void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
+  const NsPlan p = make_plan(a.rows, a.cols);
+  double* part = (double*)workspace;
+  char* ws = (char*)workspace + a.batch * kNormParts * 8;
+  const int parts = std::max(1, std::min(kNormParts, (a.rows + 15) / 16));
+  const dim3 gi((p.mp / 32) * (p.np / 32), (unsigned)a.batch), gn(parts, (unsigned)a.batch);
+  if (a.momentum.p) {
+    hipLaunchKernelGGL((ns_norm_kernel<T, true>), gn, dim3(256), 0, s, a, part);
+    hipLaunchKernelGGL((ns_init_kernel<T, true>), gi, dim3(256), 0, s, a, p, parts, part, ws);
+  } else {
+    hipLaunchKernelGGL((ns_norm_kernel<T, false>), gn, dim3(256), 0, s, a, part);
+    hipLaunchKernelGGL((ns_init_kernel<T, false>), gi, dim3(256), 0, s, a, p, parts, part, ws);
+  }
+  const int tm = (p.mp + 127) / 128, tn = (p.np + 127) / 128;
+  int cur = 0;
+  for (int k = 0; k < a.steps; ++k, cur ^= 1) {
+    char *xr = ws + p.x[cur], *xc = xr + 2 * p.xplane, *yr = ws + p.x[cur ^ 1], *yc = yr + 2 * p.xplane;
+    NsProd g{};
+    g.stride = p.stride;
+    // A = X X^T
+    g.P = g.Q = xr;
+    g.p_lo = g.q_lo = p.xplane;
+    g.Rp = g.Rq = p.mp;
+    g.K = p.np;
+    g.ti = g.tj = tm;
+    g.tiles = tm * (tm + 1) / 2;
+    g.Y = g.Z = ws + p.a;
+    g.y_lo = g.z_lo = p.aplane;
+    g.f = kSa / (kSx * kSx);
+    launch_prod<kGram, kOpF32>(g, a, p, s);
+    // B = b A + c A A
+    g.P = g.Q = g.E = ws + p.a;
+    g.p_lo = g.q_lo = g.e_lo = p.aplane;
+    g.K = p.mp;
+    g.Y = g.Z = ws + p.b;
+    g.f = a.c * kSb / (kSa * kSa);
+    g.e = a.b * kSb / kSa;
+    launch_prod<kSquare, kOpF32>(g, a, p, s);
+    // X <- a X + B X
+    g.P = ws + p.b;
+    g.Q = g.E = xc;
+    g.q_lo = g.e_lo = p.xplane;
+    g.Rq = p.np;
+    g.tj = tn;
+    g.tiles = tm * tn;
+    g.Y = yc;
+    g.Z = yr;
+    g.y_lo = g.z_lo = p.xplane;
+    const bool last = k + 1 == a.steps;
+    const float sy = last ? 1.f : kSx;
+    g.f = sy / (kSb * kSx);
+    g.e = a.a * sy / kSx;
+    if (last) launch_prod<kFinal, T>(g, a, p, s);
+    else launch_prod<kUpdate, kOpF32>(g, a, p, s);
+  }
+}
+
+}  // namespace
+
+int64_t ns_workspace(int64_t batch, int64_t rows, int64_t cols) {
+  if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+  return batch * (kNormParts * 8 + make_plan(rows, cols).stride);
+}
+
+void launch_ns(const NsArgs& a, void* workspace, hipStream_t s) {
+  // T: the type read (and, by orthogonalize, written); the parameter of muon is fp32
+  if (a.dtype == kOpF32) launch_ns_t<kOpF32>(a, workspace, s);
+  else if (a.dtype == kOpBF16) launch_ns_t<kOpBF16>(a, workspace, s);
+  else launch_ns_t<kOpF16>(a, workspace, s);
+}
+
+}  // namespace lcn

@@ -19,7 +19,7 @@ LCN_ABI_VERSION = 2
 MASK_LOCALLY_CONNECTED, MASK_EXPONENTIAL = 0, 1
 IN_DEVICE, OUT_DEVICE, NO_UPDATE, KEEP_GRADS, ASYNC = 1, 2, 4, 8, 16
 K_GEMM_FWD, K_GEMM_DX, K_GEMM_DW, K_BN_ACT, K_LIFT, K_OUT, K_OUT_DW, K_COMM = 0, 1, 2, 3, 4, 5, 6, 7
-DTYPE_F32, DTYPE_F64 = 0, 1
+DTYPE_F32, DTYPE_F64, DTYPE_BF16, DTYPE_F16 = 0, 1, 2, 3
 MAX_DATASETS, MAX_COPIES = 16, 8
 AUG_NONE, AUG_FLIP, AUG_ROTATE, AUG_TRANSLATE = 0, 1, 2, 3
 
@@ -92,6 +92,16 @@ SIGNATURES = {
     "lcn_set_dropout": ([_vp, ctypes.c_float, ctypes.c_uint64], _i32),
     "lcn_eval_mpjpe": ([_i32, _i64, _f64p, _f64p, _f64p, _f64p, _f64p, _i32, _f64p], _i32),
     "lcn_eval_mpjpe_static": ([_i32, _i64, _f64p, _f64p, _f64p, _f64p, _f64p, _i32, _f64p], _i32),
+    "lcn_orthogonalize_workspace": ([_i64, _i64, _i64], _i64),
+    "lcn_orthogonalize": ([_i32, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _f32p,
+                           ctypes.c_float, _vp, _i64], _i32),
+    "lcn_muon_update": ([_i32, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                         ctypes.c_float, _vp, ctypes.c_float, ctypes.c_float, _i32, ctypes.c_float, _i32, _f32p,
+                         ctypes.c_float, _vp, _i64], _i32),
+    "lcn_int8_linear_workspace": ([_i64, _i64, _i64], _i64),
+    "lcn_int8_linear": ([_i32, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp,
+                         _i64], _i32),
+    "lcn_int8_quantize_weight": ([_i32, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _vp], _i32),
     "lcn_set_timing": ([_vp, _i32], _i32),
     "lcn_kernel_timing": ([_vp, _i32, _i64p, _f64p, _f64p], _i32),
     "lcn_debug_tensor": ([_vp, _i32, _i32, _f32p, _i64], _i32),

@@ -1,0 +1,220 @@
+"""Weight and int8 operators on torch device tensors (HIP kernels of liblcn.so).
+
+    orthogonalize(g)                     Newton-Schulz orthogonalisation of matrices
+    muon_update(param, momentum, grad)   one Muon step, in place
+    quantize_weight(w)                   a float weight as int8 rows and channel scales
+    int8_linear(x, weight, scale, bias)  product in 8-bit integers
+
+Each runs on its tensors' device and torch's current stream of that device,
+returns without synchronising, takes its scratch memory from torch's allocator
+and can be captured into a graph.  There is no CPU path: tensors on the host are
+refused.  A bad argument raises ``ValueError``, a failure of the library
+``LcnNativeError``.  cgcnn and the CLIs reach the same kernels through
+``Network.set_optimizer`` and ``Network.set_precision``.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .native import DTYPE_BF16, DTYPE_F16, DTYPE_F32, LcnNativeError, load_library
+
+MUON_COEFFICIENTS = (3.4445, -4.775, 2.0315)
+
+_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
+def _check(rc: int):
+    if rc != 0:
+        message = load_library().lcn_last_error(None).decode()
+        raise ValueError(message) if rc == -1 else LcnNativeError(f"liblcn error {rc}: {message}")
+
+
+def _size(n: int) -> int:
+    if n < 0:
+        _check(n)
+    return n
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{name} has type {t.dtype}, expected float32, bfloat16 or float16") from None
+
+
+def _expect(cond: bool, message: str):
+    if not cond:
+        raise ValueError(message)
+
+
+def _tensor(t, name: str, device=None) -> torch.Tensor:
+    _expect(isinstance(t, torch.Tensor), f"{name} is not a tensor")
+    _expect(t.is_cuda, f"{name} is on {t.device}: these operators run on the GPU only")
+    _expect(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+    _expect(not (t.requires_grad and torch.is_grad_enabled()),
+            f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad()")
+    return t
+
+
+def _matrices(t: torch.Tensor, name: str):
+    """(batch, rows, cols, batch stride, row stride) of a [rows, cols] or [batch, rows, cols] tensor."""
+    _expect(t.dim() in (2, 3), f"{name} has {t.dim()} dimensions, expected [rows, cols] or [batch, rows, cols]")
+    s = t.stride()
+    _expect(t.shape[-1] <= 1 or s[-1] == 1, f"{name}'s last dimension is not contiguous")
+    if t.dim() == 2:
+        return 1, t.shape[0], t.shape[1], 0, s[0]
+    return t.shape[0], t.shape[1], t.shape[2], s[0], s[1]
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+_coefficients = {}
+
+
+def _triple(c):
+    """The three coefficients as a C array (kept: the same few triples come again and again)."""
+    key = tuple(c)
+    a = _coefficients.get(key)
+    if a is None:
+        _expect(len(key) == 3, "coefficients are three numbers (a, b, c)")
+        a = (ctypes.c_float * 3)(*[float(v) for v in key])
+        if len(_coefficients) < 64:
+            _coefficients[key] = a
+    return a
+
+
+def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICIENTS, eps: float = 1e-7,
+                  out: torch.Tensor = None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of every matrix of g ([rows, cols] or [batch, rows, cols],
+    float32, bfloat16 or float16):
+
+        X = G / max(|G|_F, eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X
+
+    on the transpose where rows > cols.  The result has g's type; products are accurate to float32
+    whatever that is.  out: a tensor like g for the result, g itself included.  A matrix that holds an
+    infinity or a NaN gives NaN; a zero matrix gives zero."""
+    _tensor(g, "g")
+    dt = _dtype(g, "g")
+    n, r, c, sb, sr = _matrices(g, "g")
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    else:
+        _tensor(out, "out", g.device)
+        _expect(out.shape == g.shape and out.dtype == g.dtype, "out differs from g in shape or type")
+    _, _, _, ob, orow = _matrices(out, "out")
+    lib = load_library()
+    ws = torch.empty(_size(lib.lcn_orthogonalize_workspace(n, r, c)), dtype=torch.uint8, device=g.device)
+    _check(lib.lcn_orthogonalize(g.device.index, _stream(g.device), dt, n, r, c, g.data_ptr(), sb, sr, out.data_ptr(),
+                                 ob, orow, int(steps), _triple(coefficients), eps, ws.data_ptr(), ws.numel()))
+    return out
+
+
+def muon_update(param: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor, *, lr, beta: float = 0.95,
+                nesterov: bool = True, weight_decay: float = 0.0, scale: float = None, steps: int = 5,
+                coefficients=MUON_COEFFICIENTS, eps: float = 1e-7) -> None:
+    """One Muon step on matrices ([rows, cols] or [batch, rows, cols]), in place:
+
+        momentum <- beta momentum + grad;  u = grad + beta momentum (nesterov) or momentum
+        param <- (1 - lr weight_decay) param - lr scale orthogonalize(u)
+
+    param and momentum are float32, grad float32, bfloat16 or float16.  lr: a number, or a float32 device
+    tensor of one element (read when the step runs, so a captured graph follows a schedule).  scale
+    defaults to 0.2 sqrt(max(rows, cols)), which gives an update the root mean square of Adam's, so
+    Adam's learning rates carry over."""
+    _tensor(param, "param")
+    _tensor(momentum, "momentum", param.device)
+    _tensor(grad, "grad", param.device)
+    _expect(param.dtype == momentum.dtype == torch.float32, "param and momentum are float32")
+    _expect(param.shape == momentum.shape == grad.shape, "param, momentum and grad differ in shape")
+    dt = _dtype(grad, "grad")
+    n, r, c, pb, pr = _matrices(param, "param")
+    _, _, _, mb, mr = _matrices(momentum, "momentum")
+    _, _, _, gb, gr = _matrices(grad, "grad")
+    lr_ptr, lr_value = None, 0.0
+    if isinstance(lr, torch.Tensor):
+        _tensor(lr, "lr", param.device)
+        _expect(lr.dtype == torch.float32 and lr.numel() == 1, "lr as a tensor is one float32")
+        lr_ptr = lr.data_ptr()
+    else:
+        lr_value = float(lr)
+    if scale is None:
+        scale = 0.2 * math.sqrt(max(r, c))
+    lib = load_library()
+    ws = torch.empty(_size(lib.lcn_orthogonalize_workspace(n, r, c)), dtype=torch.uint8, device=param.device)
+    _check(lib.lcn_muon_update(param.device.index, _stream(param.device), dt, n, r, c, param.data_ptr(), pb, pr,
+                               momentum.data_ptr(), mb, mr, grad.data_ptr(), gb, gr, lr_value, lr_ptr, scale, beta,
+                               int(nesterov), weight_decay, int(steps), _triple(coefficients), eps, ws.data_ptr(),
+                               ws.numel()))
+
+
+def quantize_weight(w: torch.Tensor, *, channel_dim: int = 0):
+    """(int8 weight [n, k], float32 scale [n]) for int8_linear from a float weight: [n, k], or [k, n] with
+    channel_dim=1 (any strides).  scale = max |w| / 127 of a channel, weight = rint(w * (127 / max |w|))."""
+    _tensor(w, "w")
+    dt = _dtype(w, "w")
+    _expect(w.dim() == 2, f"w has {w.dim()} dimensions, expected 2")
+    _expect(channel_dim in (0, 1), "channel_dim is 0 or 1")
+    n, k = w.shape[channel_dim], w.shape[1 - channel_dim]
+    q = torch.empty(n, k, dtype=torch.int8, device=w.device)
+    scale = torch.empty(n, dtype=torch.float32, device=w.device)
+    _check(load_library().lcn_int8_quantize_weight(w.device.index, _stream(w.device), dt, n, k, w.data_ptr(),
+                                                   w.stride(channel_dim), w.stride(1 - channel_dim), q.data_ptr(),
+                                                   scale.data_ptr()))
+    return q, scale
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor = None, *,
+                out: torch.Tensor = None) -> torch.Tensor:
+    """x [..., k] (float32, bfloat16 or float16) times weight [n, k] (int8, one scale a channel):
+
+        s = max_k |x| / 127,  q = rint(x * (127 / max_k |x|))   for each token (row of x)
+        y[t, c] = (sum_k q[t, k] weight[c, k]) * s[t] * scale[c] (+ bias[c])
+
+    scale and bias are float32 [n].  The sums are exact.  A token that holds an infinity or a NaN gives
+    NaN; one below 2^-100 everywhere counts as zero.  out: [..., n] of x's type, not overlapping the inputs.
+    For tensors on two or more leading dimensions x must be viewable as [tokens, k]."""
+    _tensor(x, "x")
+    dev = x.device
+    _tensor(weight, "weight", dev)
+    _tensor(scale, "scale", dev)
+    dt = _dtype(x, "x")
+    _expect(weight.dtype == torch.int8 and weight.dim() == 2, "weight is an int8 matrix [n, k]")
+    n, k = weight.shape
+    _expect(x.dim() >= 1 and x.shape[-1] == k, f"x ends in {tuple(x.shape[-1:])}, the weight has k = {k}")
+    _expect(k <= 1 or (x.stride(-1) == 1 and weight.stride(1) == 1), "the last dimension of x and weight is not contiguous")
+    _expect(scale.dtype == torch.float32 and scale.shape == (n,) and (n <= 1 or scale.stride(0) == 1),
+            f"scale is a contiguous float32 [{n}]")
+    bias_ptr = None
+    if bias is not None:
+        _tensor(bias, "bias", dev)
+        _expect(bias.dtype == torch.float32 and bias.shape == (n,) and (n <= 1 or bias.stride(0) == 1),
+                f"bias is a contiguous float32 [{n}]")
+        bias_ptr = bias.data_ptr()
+    x2 = x if x.dim() == 2 else _rows(x, "x")
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        _tensor(out, "out", dev)
+        _expect(out.shape == shape and out.dtype == x.dtype, f"out is a {x.dtype} {tuple(shape)}")
+        _expect(n <= 1 or out.stride(-1) == 1, "out's last dimension is not contiguous")
+    out2 = out if out.dim() == 2 else _rows(out, "out")
+    tokens = x2.shape[0]
+    lib = load_library()
+    ws = torch.empty(_size(lib.lcn_int8_linear_workspace(tokens, k, n)), dtype=torch.uint8, device=dev)
+    _check(lib.lcn_int8_linear(dev.index, _stream(dev), dt, tokens, k, n, x2.data_ptr(), x2.stride(0),
+                               weight.data_ptr(), weight.stride(0), scale.data_ptr(), bias_ptr, out2.data_ptr(),
+                               out2.stride(0), ws.data_ptr(), ws.numel()))
+    return out
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    try:
+        return t.view(-1, t.shape[-1]) if t.numel() else t.new_empty(math.prod(t.shape[:-1]), t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name}'s leading dimensions cannot be viewed as one") from None
