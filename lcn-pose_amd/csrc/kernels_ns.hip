@@ -12,12 +12,14 @@
 // Precision.  The iteration amplifies a perturbation of a small singular
 // direction by up to a^steps (485 for the default): with X in one fp16 the
 // result of a rank-64 gradient is 11 bf16 roundings off.  Every matrix is
-// therefore held as two fp16 numbers, v S = hi + lo / 2048 (22 significant
-// bits), and every product is three fp16 MFMA products, hi hi + (hi lo + lo hi)
-// / 2048, summed in two fp32 accumulators; the dropped lo lo term is below
-// 2^-22 of the result.  Three products at the fp16 rate are still five times
-// the rate of the fp32 MFMA.  S is a power of two per matrix kind that keeps
-// the entries inside fp16's range (|X|, |B| <= 64, |A| <= 16).
+// therefore held as two fp16 numbers, v S = hi + lo (22 significant bits), and
+// every product is three fp16 MFMA products, hi hi + hi lo + lo hi, summed in
+// one fp32 accumulator; the dropped lo lo term is below 2^-22 of the result.
+// Three products at the fp16 rate are still five times the rate of the fp32
+// MFMA.  S is a power of two per matrix kind: as large as fp16's range allows
+// (|X| < 2, |A| < 4, |B| < 16), so that the lo halves stay clear of fp16's
+// smallest numbers (X0 of 2^30 entries has a root mean square of 1 in units of
+// 1 / S, its lo halves a spacing of 2^-24).
 //
 // Layout.  A plane (the hi or the lo half of a matrix with R rows and
 // contraction length K, both padded to 32 with zeros) is stored as
@@ -36,8 +38,7 @@ namespace lcn {
 
 namespace {
 
-constexpr float kSx = 1024.f, kSa = 4096.f, kSb = 1024.f;  // scales of X, A, B
-constexpr float kLo = 2048.f;                              // scale of the lo halves
+constexpr float kSx = 32768.f, kSa = 16384.f, kSb = 4096.f;  // scales of X, A, B
 constexpr int kNormParts = 64;                             // partial sums of squares per matrix
 
 __host__ __device__ inline int64_t pad32(int64_t v) { return (v + 31) / 32 * 32; }
@@ -68,7 +69,7 @@ NsPlan make_plan(int64_t rows, int64_t cols) {
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
-  lo = (_Float16)((v - (float)hi) * kLo);
+  lo = (_Float16)(v - (float)hi);
 }
 
 // ---- norm (and, for muon, the momentum update) ---------------------------------------------
@@ -170,14 +171,20 @@ struct NsProd {
 
 #define NS_LDS(SRC, VOFF, SOFF, DST) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
+// waits until at most N of this wave's loads are outstanding
+#define NS_WAIT(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | 0x0f70)
 
-// One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 32
-// through a double LDS buffer filled by LDS-DMA (32 KB a stage: hi and lo of
-// both operands).  All fragments of a stage are read before the next stage's
-// loads are issued, so no LDS read waits for them.
+// One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 16
+// through a ring of four LDS buffers filled by LDS-DMA (16 KB a stage: hi and
+// lo of both operands), three stages in flight: with one stage in flight a
+// lone workgroup of a CU spent three quarters of its time waiting for the next
+// (46 us for six 1088 x 1088 Gram matrices).  The buffers are four LDS objects, and
+// a stage's object is known at compile time, so the compiler adds no waits of
+// its own for loads into the others.
 template <int MODE, int T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void ns_prod_kernel(NsProd g, NsArgs a, NsPlan pl) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * 32768];
+  constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
+  __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int mat = id / g.tiles, t = id - mat * g.tiles;
   int ti, tj;
@@ -204,54 +211,82 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
-  // stage layout: P hi | P lo | Q hi | Q lo, 8 KB each = 4 row blocks x 2 KB
-  auto stage = [&](int ks, int buf) {
-    char* d = lds + buf * 32768 + w * 2048;
-    const int so = ks * 2048;
-    NS_LDS(rph, vo, so, d);                NS_LDS(rph, vo, so + 1024, d + 1024);
-    NS_LDS(rpl, vo, so, d + 8192);         NS_LDS(rpl, vo, so + 1024, d + 8192 + 1024);
-    NS_LDS(rqh, vo, so, d + 16384);        NS_LDS(rqh, vo, so + 1024, d + 16384 + 1024);
-    NS_LDS(rql, vo, so, d + 24576);        NS_LDS(rql, vo, so + 1024, d + 24576 + 1024);
+  // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = 4 row blocks x 1 KB
+  auto stage = [&](int ks, char* buf) {
+    char* d = buf + w * 1024;
+    const int so = ks * 1024;
+    NS_LDS(rph, vo, so, d);
+    NS_LDS(rpl, vo, so, d + 4096);
+    NS_LDS(rqh, vo, so, d + 8192);
+    NS_LDS(rql, vo, so, d + 12288);
   };
-  f32x16 acc[2][2], cr[2][2];
+  f32x16 acc[2][2];
 #pragma unroll
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) { acc[x][y][e] = 0.f; cr[x][y][e] = 0.f; }
-  const int nk = g.K / 32;
-  stage(0, 0);
-  __syncthreads();
-  for (int ks = 0; ks < nk; ++ks) {
-    const char* s = lds + (ks & 1) * 32768;
-    half8 ph[2][2], plo[2][2], qh[2][2], qlo[2][2];  // [row block][k16]
+      for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
+  const int nk = g.K / 16;  // even
+  // stage s: its loads have landed (this wave's by the wait, the others' by the
+  // barrier), every wave has read stage s - 1 -- so its buffer takes stage s + 3
+  auto step = [&](int s, const char* buf, char* next, bool full) {
+    if (full) NS_WAIT((R - 2) * L);
+    else NS_WAIT(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (full) stage(s + R - 1, next);
+    half8 ph[2], plo[2], qh[2], qlo[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int op = (wi * 2 + x) * 1024 + vo, oq = (wj * 2 + x) * 1024 + vo;
+      ph[x] = *(const half8*)(buf + op);
+      plo[x] = *(const half8*)(buf + 4096 + op);
+      qh[x] = *(const half8*)(buf + 8192 + oq);
+      qlo[x] = *(const half8*)(buf + 12288 + oq);
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int op = (wi * 2 + x) * 2048 + kk * 1024 + vo, oq = (wj * 2 + x) * 2048 + kk * 1024 + vo;
-        ph[x][kk] = *(const half8*)(s + op);
-        plo[x][kk] = *(const half8*)(s + 8192 + op);
-        qh[x][kk] = *(const half8*)(s + 16384 + oq);
-        qlo[x][kk] = *(const half8*)(s + 24576 + oq);
-      }
-    __builtin_amdgcn_sched_barrier(0);
-    if (ks + 1 < nk) stage(ks + 1, (ks + 1) & 1);
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], qh[y], acc[x][y], 0, 0, 0);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], qlo[y], acc[x][y], 0, 0, 0);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x][kk], qh[y][kk], acc[x][y], 0, 0, 0);
-          cr[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x][kk], qlo[y][kk], cr[x][y], 0, 0, 0);
-          cr[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(plo[x][kk], qh[y][kk], cr[x][y], 0, 0, 0);
-        }
-    __syncthreads();
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(plo[x], qh[y], acc[x][y], 0, 0, 0);
+    asm volatile("" ::: "memory");
+  };
+  int ks = 0;
+  if (nk >= 2 * R - 1) {  // (a block of its own: the compiler then knows how many loads are outstanding in the loop)
+    stage(0, l0);
+    stage(1, l1);
+    stage(2, l2);
+    do {  // every step has a stage left to load
+      step(ks, l0, l3, true);
+      step(ks + 1, l1, l0, true);
+      step(ks + 2, l2, l1, true);
+      step(ks + 3, l3, l2, true);
+      ks += R;
+    } while (ks + 2 * R - 1 <= nk);
+  } else {
+    stage(0, l0);
+    if (nk > 1) stage(1, l1);
+    if (nk > 2) stage(2, l2);
   }
-  // epilogue, one 32 x 32 block at a time; the wave transposes in its own 4.2 KB of LDS
-  unsigned* tr = (unsigned*)lds + w * (32 * 33);
+  for (; ks < nk; ks += R) {  // at most six stages remain
+    const int left = nk - ks;
+    step(ks, l0, l3, left > 3);
+    if (left > 1) step(ks + 1, l1, l0, left > 4);
+    if (left > 2) step(ks + 2, l2, l1, left > 5);
+    if (left > 3) step(ks + 3, l3, l2, left > 6);
+  }
+  __syncthreads();
+  // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
+  unsigned* tr = (unsigned*)(w == 0 ? l0 : w == 1 ? l1 : w == 2 ? l2 : l3);
   const float lr = MODE == kFinal && a.momentum.p ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -261,7 +296,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       if (rbi >= nPb || rbj >= nQb) continue;
       float v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = fmaf(cr[x][y][e], 1.f / kLo, acc[x][y][e]) * g.f;
+      for (int e = 0; e < 16; ++e) v[e] = acc[x][y][e] * g.f;
       // (row j, contraction i): octet 4 rbi + q of row block rbj, row l31, halves 4h .. 4h + 3
       const int64_t at = (((int64_t)rbj * (g.Rp / 8) + rbi * 4) * 32 + l31) * 16 + h * 8;
       if constexpr (MODE != kGram) {
@@ -270,7 +305,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
         for (int q = 0; q < 4; ++q) {
           const half4 eh = *(const half4*)(E + q * 512), el = *(const half4*)(E + g.e_lo + q * 512);
 #pragma unroll
-          for (int s2 = 0; s2 < 4; ++s2) v[4 * q + s2] = fmaf(fmaf((float)el[s2], 1.f / kLo, (float)eh[s2]), g.e, v[4 * q + s2]);
+          for (int s2 = 0; s2 < 4; ++s2) v[4 * q + s2] = fmaf((float)eh[s2] + (float)el[s2], g.e, v[4 * q + s2]);
         }
       }
       if constexpr (MODE == kFinal) {
