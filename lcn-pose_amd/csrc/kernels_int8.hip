@@ -30,28 +30,106 @@ __device__ __forceinline__ int quant(float v, float factor) {
   return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
-// one wave a row: largest magnitude, then the integers, rows padded to kp with zeros
+// 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
+template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
 template <int T>
+__device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {
+  const v4u u = *(const v4u*)((const char*)p + e * (16 / kVec<T>));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == kOpF32) v[i] = __uint_as_float(u[i]);
+    else if constexpr (T == kOpBF16) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    else {
+      v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)u[i]);
+      v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
+    }
+  }
+}
+// largest magnitude of a wave's values, and whether one is an infinity or a NaN
+__device__ __forceinline__ void wave_top(float& top, bool& bad) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  bad = __any(bad);
+}
+__device__ __forceinline__ void see(float v, float& top, bool& bad) {
+  v = fabsf(v);
+  bad |= !(v < __builtin_inff());
+  top = fmaxf(top, v);
+}
+
+// One wave a row: largest magnitude, then the integers, rows padded to kp with
+// zeros.  kAligned: rows of whole 16-byte pieces; up to kRegs pieces a lane stay
+// in registers between the two passes, the rest is read again (from L2).
+// Bound by the read of x: 65 536 x 1088 fp32 in .. us.
+template <int T, bool kAligned>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict__ x, int64_t x_row, int64_t tokens, int k,
                                                          int64_t kp, int8_t* __restrict__ q, float* __restrict__ scale) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (t >= tokens) return;
-  float top = 0.f;
+  float top = 0.f, factor, s;
   bool bad = false;
-  for (int c = lane; c < k; c += 64) {
-    const float v = fabsf(op_load<T>(x, t * x_row + c));
-    bad |= !(v < __builtin_inff());
-    top = fmaxf(top, v);
-  }
+  const int64_t r = t * x_row;
+  int8_t* out = q + t * kp;
+  if constexpr (kAligned) {
+    constexpr int V = kVec<T>, kRegs = 6;
+    const int pieces = k / V;  // k is a multiple of V here
+    float keep[kRegs][V];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  bad = __any(bad);
-  float factor, s;
-  row_scale(top, bad, factor, s);
+    for (int i = 0; i < kRegs; ++i) {
+      if (lane + 64 * i < pieces) load_vec<T>(x, r + (int64_t)(lane + 64 * i) * V, keep[i]);
+      else
+#pragma unroll
+        for (int e = 0; e < V; ++e) keep[i][e] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) see(keep[i][e], top, bad);
+    for (int c = lane + 64 * kRegs; c < pieces; c += 64) {
+      float v[V];
+      load_vec<T>(x, r + (int64_t)c * V, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) see(v[e], top, bad);
+    }
+    wave_top(top, bad);
+    row_scale(top, bad, factor, s);
+    auto put = [&](int c, const float (&v)[V]) {
+      unsigned w[V / 4];
+#pragma unroll
+      for (int d = 0; d < V / 4; ++d) {
+        w[d] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[d] |= (bad ? 0u : (unsigned)(quant(v[4 * d + e], factor) & 255)) << (8 * e);
+      }
+      if constexpr (V == 4) *(unsigned*)(out + (int64_t)c * 4) = w[0];
+      else *(uint2*)(out + (int64_t)c * 8) = make_uint2(w[0], w[1]);
+    };
+    const int padded = (int)(kp / V);  // the pieces past k hold zeros
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (lane + 64 * i < padded) put(lane + 64 * i, keep[i]);
+    for (int c = lane + 64 * kRegs; c < padded; c += 64) {
+      float v[V] = {};
+      if (c < pieces) load_vec<T>(x, r + (int64_t)c * V, v);
+      put(c, v);
+    }
+  } else {
+    constexpr int kRegs = 16;
+    float keep[kRegs];
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) keep[i] = lane + 64 * i < k ? op_load<T>(x, r + lane + 64 * i) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) see(keep[i], top, bad);
+    for (int c = lane + 64 * kRegs; c < k; c += 64) see(op_load<T>(x, r + c), top, bad);
+    wave_top(top, bad);
+    row_scale(top, bad, factor, s);
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (lane + 64 * i < kp) out[lane + 64 * i] = bad ? (int8_t)0 : (int8_t)quant(keep[i], factor);
+    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[c] = c < k && !bad ? (int8_t)quant(op_load<T>(x, r + c), factor) : (int8_t)0;
+  }
   if (lane == 0) scale[t] = s;
-  for (int64_t c = lane; c < kp; c += 64)
-    q[t * kp + c] = c < k && !bad ? (int8_t)quant(op_load<T>(x, t * x_row + c), factor) : (int8_t)0;
 }
 
 // weight rows of any alignment -> rows of kp bytes, zero padded
@@ -73,84 +151,218 @@ struct Int8Gemm {
   int tn;                                          // channel tiles
 };
 
-// 128 tokens x 128 channels, four waves of 64 x 64, 64 bytes of K a stage
-// through a double LDS buffer.  A stage holds rows of 64 bytes (four 16-byte
-// units); unit c of row r sits at c ^ ((r >> 2) & 3), so the 32 rows of a
-// fragment read spread over all banks; the permutation is made by the lane's
-// choice of global address.
-template <int T>
+// A tile of 64 BI tokens x 64 BJ channels, 2 x 2 waves of 32 BI x 32 BJ, 64
+// bytes of K a stage through a ring of R LDS buffers filled by LDS-DMA, R - 1
+// stages in flight.  A stage holds rows of 64 bytes (four 16-byte units); unit c
+// of row r sits at c ^ ((r >> 2) & 3), so the 32 rows of a fragment read spread
+// over all banks; the permutation is made by the lane's choice of global
+// address.  The buffers are separate LDS objects, so the compiler adds no waits
+// for loads into the others.
+template <int T, int BI, int BJ, int R>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void int8_gemm_kernel(Int8Gemm g) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * 16384];
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass emits no launch stub for this body)
+  constexpr int kRows = 64 * (BI + BJ), kStage = kRows * 64, L = BI + BJ;  // L: loads of a wave per stage
+  static_assert(R == 3 || R == 4, "ring depth");
+  __shared__ __attribute__((aligned(16))) char l0[kStage], l1[kStage], l2[kStage], l3[R == 4 ? kStage : 16];
   const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int64_t t0 = (int64_t)(id / g.tn) * 128;
-  const int n0 = (id % g.tn) * 128;
+  const int64_t t0 = (int64_t)(id / g.tn) * (64 * BI);
+  const int n0 = (id % g.tn) * (64 * BJ);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = w >> 1, wj = w & 1, h = lane >> 5, l31 = lane & 31;
   // rows past the end repeat the last one; their results are not stored
-  const int trows = (int)min((int64_t)128, g.tokens - t0), nrows = min(128, g.n - n0);
+  const int trows = (int)min((int64_t)(64 * BI), g.tokens - t0), nrows = min(64 * BJ, g.n - n0);
   const int64_t qbytes = (int64_t)trows * g.kp, wbytes = (int64_t)(nrows - 1) * g.w_row + g.kw;
   const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(g.q + t0 * g.kp), 0, (int)qbytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + n0 * g.w_row), 0, (int)wbytes, 0x00020000);
-  int voq[2], vow[2];
+  // load i of a wave: 16 rows x 64 bytes
+  int voq[BI], vow[BJ];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = w * 32 + i * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 2) & 3);
-    voq[i] = min(r, trows - 1) * (int)g.kp + c * 16;
-    vow[i] = min(r, nrows - 1) * (int)g.w_row + c * 16;
+  for (int i = 0; i < BI; ++i) {
+    const int r = (i * 4 + w) * 16 + (lane >> 2);
+    voq[i] = min(r, trows - 1) * (int)g.kp + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
   }
-  auto stage = [&](int ks, int buf) {
-    char* d = lds + buf * 16384 + w * 2048;
+#pragma unroll
+  for (int i = 0; i < BJ; ++i) {
+    const int r = (i * 4 + w) * 16 + (lane >> 2);
+    vow[i] = min(r, nrows - 1) * (int)g.w_row + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
+  }
+  auto stage = [&](int ks, char* buf) {
+    char* d = buf + w * 1024;
     const int so = ks * 64;
-    I8_LDS(rq, voq[0], so, d);        I8_LDS(rq, voq[1], so, d + 1024);
-    I8_LDS(rw, vow[0], so, d + 8192); I8_LDS(rw, vow[1], so, d + 8192 + 1024);
+#pragma unroll
+    for (int i = 0; i < BI; ++i) I8_LDS(rq, voq[i], so, d + i * 4096);
+#pragma unroll
+    for (int i = 0; i < BJ; ++i) I8_LDS(rw, vow[i], so, d + (BI + i) * 4096);
   };
-  v16i acc[2][2];
+  v16i acc[BI][BJ];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < BI; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < BJ; ++y)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0;
   const int nk = (int)(g.kp / 64);
-  stage(0, 0);
-  __syncthreads();
-  for (int ks = 0; ks < nk; ++ks) {
-    const char* s = lds + (ks & 1) * 16384;
-    v4i p[2][2], q[2][2];
+  // stage s has landed (this wave's loads by the wait, the others' by the
+  // barrier) and every wave has read stage s - 1, whose buffer takes s + R - 1
+  auto step = [&](int s, const char* buf, char* next, bool full) {
+    if (full) wait_loads<(R - 2) * L>();
+    else wait_loads<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (full) stage(s + R - 1, next);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int kk = 0; kk < 2; ++kk) {
+      v4i p[BI], q[BJ];
+      const int c = ((2 * kk + h) ^ ((l31 >> 2) & 3)) * 16 + l31 * 64;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const int rp = wi * 64 + x * 32 + l31, rw_ = wj * 64 + x * 32 + l31, c = (2 * kk + h) ^ ((l31 >> 2) & 3);
-        p[x][kk] = *(const v4i*)(s + rp * 64 + c * 16);
-        q[x][kk] = *(const v4i*)(s + 8192 + rw_ * 64 + c * 16);
+      for (int x = 0; x < BI; ++x) p[x] = *(const v4i*)(buf + (wi * BI + x) * 2048 + c);
+#pragma unroll
+      for (int y = 0; y < BJ; ++y) q[y] = *(const v4i*)(buf + BI * 4096 + (wj * BJ + y) * 2048 + c);
+#pragma unroll
+      for (int x = 0; x < BI; ++x)
+#pragma unroll
+        for (int y = 0; y < BJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(p[x], q[y], acc[x][y], 0, 0, 0);
+    }
+    asm volatile("" ::: "memory");
+  };
+  int ks = 0;
+  if (nk >= 2 * R - 1) {
+    stage(0, l0);
+    stage(1, l1);
+    if constexpr (R == 4) stage(2, l2);
+    do {
+      if constexpr (R == 4) {
+        step(ks, l0, l3, true);
+        step(ks + 1, l1, l0, true);
+        step(ks + 2, l2, l1, true);
+        step(ks + 3, l3, l2, true);
+      } else {
+        step(ks, l0, l2, true);
+        step(ks + 1, l1, l0, true);
+        step(ks + 2, l2, l1, true);
       }
-    __builtin_amdgcn_sched_barrier(0);
-    if (ks + 1 < nk) stage(ks + 1, (ks + 1) & 1);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(p[x][kk], q[y][kk], acc[x][y], 0, 0, 0);
-    __syncthreads();
+      ks += R;
+    } while (ks + 2 * R - 1 <= nk);
+  } else {
+    stage(0, l0);
+    if (nk > 1) stage(1, l1);
+    if (R == 4 && nk > 2) stage(2, l2);
+  }
+  for (; ks < nk; ks += R) {
+    const int left = nk - ks;
+    if constexpr (R == 4) {
+      step(ks, l0, l3, left > 3);
+      if (left > 1) step(ks + 1, l1, l0, left > 4);
+      if (left > 2) step(ks + 2, l2, l1, left > 5);
+      if (left > 3) step(ks + 3, l3, l2, left > 6);
+    } else {
+      step(ks, l0, l2, left > 2);
+      if (left > 1) step(ks + 1, l1, l0, left > 3);
+      if (left > 2) step(ks + 2, l2, l1, left > 4);
+    }
   }
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    const int n = n0 + wj * 64 + y * 32 + l31;
+  for (int y = 0; y < BJ; ++y) {
+    const int n = n0 + (wj * BJ + y) * 32 + l31;
     if (n >= g.n) continue;
     const float sw = g.ws[n], b = g.bias ? g.bias[n] : 0.f;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < BI; ++x)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t t = t0 + wi * 64 + x * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-        if (t >= g.tokens) continue;
-        float v = (float)acc[x][y][e] * g.qs[t] * sw;
-        if (g.bias) v += b;
-        op_store<T>(g.out, t * g.out_row + n, v);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t t = t0 + (wi * BI + x) * 32 + 8 * q + 4 * h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (t + e >= g.tokens) continue;
+          float v = (float)acc[x][y][4 * q + e] * g.qs[t + e] * sw;
+          if (g.bias) v += b;
+          op_store<T>(g.out, (t + e) * g.out_row + n, v);
+        }
       }
+  }
+#endif
+}
+
+// ---- few tokens ----------------------------------------------------------------------------
+// At most 16 tokens: a workgroup takes 16 channels, its four waves every fourth
+// 64-byte piece of K, straight from memory into v_mfma_i32_16x16x64_i8; the
+// partial sums meet in LDS.  kFused: the workgroup also quantises the tokens,
+// each time anew (they are small), which makes the product one launch.  Bound by
+// latency: one round of loads in flight for the weights.
+constexpr int kFewTokens = 16;
+constexpr int kFewLds = 65536;   // bytes of quantised tokens a workgroup holds
+
+template <int T, bool kFused, bool kAligned>
+__global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ int red[4][256];
+  __shared__ float qs[kFewTokens];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int kp = (int)g.kp, tokens = (int)g.tokens;
+  const int n0 = blockIdx.x * 16;
+  const int c16 = lane & 15, kq = lane >> 4;  // channel (or token) of the fragment, its 16-byte quarter of a piece
+  const int8_t* wrow = g.w + (int64_t)min(n0 + c16, g.n - 1) * g.w_row;
+  auto weights = [&](int ks) {
+    const int at = ks * 64 + kq * 16;
+    v4i v = {0, 0, 0, 0};
+    if constexpr (kAligned) {
+      // a 16-byte piece may end past the row: it stays inside it where k is a multiple of 16
+      if (at < k) v = *(const v4i*)(wrow + at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (at + e < k) v[e >> 2] |= (int)((unsigned)(uint8_t)wrow[at + e] << (8 * (e & 3)));
+    }
+    return v;
+  };
+  const int nk = kp / 64;
+  constexpr int kAhead = 4;  // pieces of a wave in flight
+  v4i wv[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (w + 4 * i < nk) wv[i] = weights(w + 4 * i);
+  const int pitch = kp + 16;  // rows start 16 bytes apart in the banks
+  if constexpr (kFused) {
+    for (int t = w; t < tokens; t += 4) {
+      float top = 0.f, factor, s;
+      bool bad = false;
+      for (int c = lane; c < k; c += 64) see(op_load<T>(x, t * x_row + c), top, bad);
+      wave_top(top, bad);
+      row_scale(top, bad, factor, s);
+      if (lane == 0) qs[t] = s;
+      for (int c = lane; c < kp; c += 64)
+        lds[t * pitch + c] = c < k && !bad ? (char)quant(op_load<T>(x, t * x_row + c), factor) : (char)0;
+    }
+    __syncthreads();
+  } else if (threadIdx.x < tokens) {
+    qs[threadIdx.x] = g.qs[threadIdx.x];
+  }
+  v4i acc = {0, 0, 0, 0};
+  const int tr = min(c16, tokens - 1);  // rows past the tokens repeat the last
+  for (int ks = w; ks < nk; ks += 4 * kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int p = ks + 4 * i;
+      if (p >= nk) break;
+      v4i q;
+      if constexpr (kFused) q = *(const v4i*)(lds + tr * pitch + p * 64 + kq * 16);
+      else q = *(const v4i*)(g.q + (int64_t)tr * kp + p * 64 + kq * 16);
+      const v4i ww = wv[i];
+      if (p + 4 * kAhead < nk) wv[i] = weights(p + 4 * kAhead);
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q, ww, acc, 0, 0, 0);
+    }
+  }
+  // lane holds tokens 4 kq .. 4 kq + 3 of channel c16
+#pragma unroll
+  for (int e = 0; e < 4; ++e) red[w][(4 * kq + e) * 16 + c16] = acc[e];
+  __syncthreads();
+  const int t = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15);
+  if (t < tokens && n < g.n) {
+    const int sum = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+    float v = (float)sum * qs[t] * g.ws[n];
+    if (g.bias) v += g.bias[n];
+    op_store<T>(g.out, t * g.out_row + n, v);
   }
 }
 
@@ -177,6 +389,22 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWArgs a) {
 }
 
 template <int T>
+void launch_quant_rows(const Int8Args& a, int64_t kp, int8_t* q, float* qs, hipStream_t s) {
+  constexpr int V = kVec<T>;
+  const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && (a.x_row % V == 0 || a.tokens == 1);
+  const dim3 grid((unsigned)((a.tokens + 3) / 4));
+  if (al) hipLaunchKernelGGL((quant_rows_kernel<T, true>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  else hipLaunchKernelGGL((quant_rows_kernel<T, false>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+}
+
+template <int T, int BI, int BJ, int R>
+void launch_tiles(Int8Gemm& g, hipStream_t s) {
+  g.tn = (g.n + 64 * BJ - 1) / (64 * BJ);
+  const int64_t tt = (g.tokens + 64 * BI - 1) / (64 * BI);
+  hipLaunchKernelGGL((int8_gemm_kernel<T, BI, BJ, R>), dim3((unsigned)(tt * g.tn)), dim3(256), 0, s, g);
+}
+
+template <int T>
 void launch_int8_t(const Int8Args& a, void* workspace, hipStream_t s) {
   const int64_t kp = pad64(a.k);
   char* p = (char*)workspace;
@@ -185,10 +413,28 @@ void launch_int8_t(const Int8Args& a, void* workspace, hipStream_t s) {
   int8_t* q = (int8_t*)p;
   p += pad256(a.tokens * kp);
   int8_t* wp = (int8_t*)p;
-  hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)((a.tokens + 3) / 4)), dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
   Int8Gemm g{};
   g.q = q; g.qs = qs; g.kp = kp;
   g.w = a.w; g.w_row = a.w_row; g.kw = a.k;
+  g.ws = a.w_scale; g.bias = a.bias;
+  g.out = a.out; g.out_row = a.out_row;
+  g.tokens = a.tokens; g.n = a.n;
+  if (a.tokens <= kFewTokens) {
+    const bool al = a.k % 16 == 0 && a.w_row % 16 == 0 && (uintptr_t)a.w % 16 == 0;
+    const int64_t lds = a.tokens * (kp + 16);
+    const dim3 grid((a.n + 15) / 16);
+    // every workgroup quantises the tokens for itself while that is little work
+    if (lds <= kFewLds && a.tokens * a.k <= 16384) {
+      if (al) hipLaunchKernelGGL((int8_few_kernel<T, true, true>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
+      else hipLaunchKernelGGL((int8_few_kernel<T, true, false>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
+    } else {
+      launch_quant_rows<T>(a, kp, q, qs, s);
+      if (al) hipLaunchKernelGGL((int8_few_kernel<T, false, true>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
+      else hipLaunchKernelGGL((int8_few_kernel<T, false, false>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
+    }
+    return;
+  }
+  launch_quant_rows<T>(a, kp, q, qs, s);
   // rows that 16-byte loads at 32-bit offsets cannot address are laid out again
   // (k % 4: the loads' bounds check drops a dword that ends past the last row)
   if (a.k % 4 || a.w_row % 16 || (uintptr_t)a.w % 16 || a.w_row > (1 << 20)) {
@@ -196,11 +442,10 @@ void launch_int8_t(const Int8Args& a, void* workspace, hipStream_t s) {
     g.w = wp;
     g.w_row = g.kw = kp;
   }
-  g.ws = a.w_scale; g.bias = a.bias;
-  g.out = a.out; g.out_row = a.out_row;
-  g.tokens = a.tokens; g.n = a.n;
-  g.tn = (a.n + 127) / 128;
-  hipLaunchKernelGGL((int8_gemm_kernel<T>), dim3((unsigned)((a.tokens + 127) / 128 * g.tn)), dim3(256), 0, s, g);
+  const int64_t t256 = (a.tokens + 255) / 256 * ((a.n + 127) / 128), t128 = (a.tokens + 127) / 128 * ((a.n + 127) / 128);
+  if (t256 >= 512) launch_tiles<T, 4, 2, 3>(g, s);
+  else if (t128 >= 256) launch_tiles<T, 2, 2, 4>(g, s);
+  else launch_tiles<T, 1, 1, 4>(g, s);
 }
 
 }  // namespace

@@ -39,7 +39,7 @@ namespace lcn {
 namespace {
 
 constexpr float kSx = 32768.f, kSa = 16384.f, kSb = 4096.f;  // scales of X, A, B
-constexpr int kNormParts = 64;                             // partial sums of squares per matrix
+constexpr int kNormParts = 512;                             // most partial sums of squares per matrix
 
 __host__ __device__ inline int64_t pad32(int64_t v) { return (v + 31) / 32 * 32; }
 
@@ -73,7 +73,10 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
 }
 
 // ---- norm (and, for muon, the momentum update) ---------------------------------------------
-// part[b][p] = sum of squares, in float64, of the rows this workgroup walks.
+// part[b][p] = sum of squares, in float64, of the rows this workgroup walks.  A
+// wave takes a row at a time, 64 x kU elements in flight; bound by the read of
+// G (six 1088 x 1088: 28 us with one element in flight and 64 workgroups).
+constexpr int kU = 8;
 template <int T, bool kMuon>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restrict__ part) {
   __shared__ double red[4];
@@ -83,14 +86,23 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restri
   for (int r = blockIdx.x * 4 + ty; r < a.rows; r += gridDim.x * 4) {
     const int64_t g0 = b * a.in.batch + (int64_t)r * a.in.row;
     float* mom = kMuon ? (float*)a.momentum.p + b * a.momentum.batch + (int64_t)r * a.momentum.row : nullptr;
-    for (int c = tx; c < a.cols; c += 64) {
-      float v = op_load<T>(a.in.p, g0 + c);
-      if constexpr (kMuon) {
-        const float m = fmaf(a.beta, mom[c], v);
-        mom[c] = m;
-        v = a.nesterov ? fmaf(a.beta, m, v) : m;
+    for (int c0 = tx; c0 < a.cols; c0 += 64 * kU) {
+      float v[kU], m[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int c = c0 + 64 * u;
+        v[u] = c < a.cols ? op_load<T>(a.in.p, g0 + c) : 0.f;
+        if constexpr (kMuon) m[u] = c < a.cols ? mom[c] : 0.f;
       }
-      s += (double)v * (double)v;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if constexpr (kMuon) {
+          m[u] = fmaf(a.beta, m[u], v[u]);
+          if (c0 + 64 * u < a.cols) mom[c0 + 64 * u] = m[u];
+          v[u] = a.nesterov ? fmaf(a.beta, m[u], v[u]) : m[u];
+        }
+        s = fma((double)v[u], (double)v[u], s);
+      }
     }
   }
 #pragma unroll
@@ -98,6 +110,15 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restri
   if (tx == 0) red[ty] = s;
   __syncthreads();
   if (threadIdx.x == 0) part[b * kNormParts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// the matrix's sum of squares from its partials, in every lane of a wave
+__device__ __forceinline__ double norm2_of(const double* __restrict__ part, int parts) {
+  double s = 0.0;
+  for (int q = threadIdx.x & 63; q < parts; q += 64) s += part[q];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  return s;
 }
 
 // ---- X0 in both orientations ---------------------------------------------------------------
@@ -108,10 +129,7 @@ __global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, NsPlan p, int pa
   const int64_t b = blockIdx.y;
   const int nb = p.np / 32;
   const int bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;  // 32-row block of X, 32-column block
-  const int lane = threadIdx.x & 63;
-  double s = lane < parts ? part[b * kNormParts + lane] : 0.0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  const double s = norm2_of(part + b * kNormParts, parts);
   const double inv = (double)kSx / fmax(sqrt(s), (double)a.eps);
   const bool bad = !(s < 1e300);  // an infinity or a NaN in the matrix: every entry becomes NaN
   const bool tall = a.rows > a.cols;
@@ -161,8 +179,8 @@ struct NsProd {
   int64_t p_lo, q_lo;
   int Rp, Rq, K;                      // rows (multiples of 32) of P and Q, contraction length
   int64_t stride;                     // bytes between the matrices' workspaces
-  int ti, tj;                         // 128-row tiles of P and Q
-  int tiles;                          // tiles of a matrix
+  int ti, tj;                         // 128-row tiles of P and Q that are whole
+  int whole, rest;                    // tiles of a matrix: whole ones, ones with a partial row block
   const char* E; int64_t e_lo;        // kSquare: A (= Q); kUpdate / kFinal: Xc, in (row j, contraction i) form
   char* Y; int64_t y_lo;              // result in (row j, contraction i) form
   char* Z; int64_t z_lo;              // result in (row i, contraction j) form
@@ -171,8 +189,6 @@ struct NsProd {
 
 #define NS_LDS(SRC, VOFF, SOFF, DST) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
-// waits until at most N of this wave's loads are outstanding
-#define NS_WAIT(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | 0x0f70)
 
 // One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 16
 // through a ring of four LDS buffers filled by LDS-DMA (16 KB a stage: hi and
@@ -185,17 +201,27 @@ template <int MODE, int T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void ns_prod_kernel(NsProd g, NsArgs a, NsPlan pl) {
   constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
   __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int mat = id / g.tiles, t = id - mat * g.tiles;
+  // The whole tiles of all matrices come first, then those with fewer than four
+  // row blocks of either operand (whose idle waves return the CU to others).
+  const int nwhole = g.whole * (int)a.batch;
+  const bool rest = (int)blockIdx.x >= nwhole;
+  const int id = rest ? xcd_remap(blockIdx.x - nwhole, gridDim.x - nwhole) : xcd_remap(blockIdx.x, nwhole);
+  const int mat = id / (rest ? g.rest : g.whole);
+  int t = id - mat * (rest ? g.rest : g.whole);
   int ti, tj;
-  if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle: ti >= tj
+  if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle, ti >= tj, row after row
+    if (rest) t += g.whole;
     ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > t) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
     tj = t - ti * (ti + 1) / 2;
-  } else {
+  } else if (!rest) {
     ti = t % g.ti;
     tj = t / g.ti;
+  } else {  // the last column of tiles, if partial, then the last row
+    const int side = g.Rq / 32 > g.tj * 4 ? g.ti : 0;
+    ti = t < side ? t : g.ti;
+    tj = t < side ? g.tj : t - side;
   }
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = w >> 1, wj = w & 1, h = lane >> 5, l31 = lane & 31;
@@ -211,6 +237,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
+  const bool live = ti * 4 + wi * 2 < nPb && tj * 4 + wj * 2 < nQb;  // any block of this wave's 64 x 64 in range
   // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = 4 row blocks x 1 KB
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
@@ -231,12 +258,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   // stage s: its loads have landed (this wave's by the wait, the others' by the
   // barrier), every wave has read stage s - 1 -- so its buffer takes stage s + 3
   auto step = [&](int s, const char* buf, char* next, bool full) {
-    if (full) NS_WAIT((R - 2) * L);
-    else NS_WAIT(0);
+    if (full) wait_loads<(R - 2) * L>();
+    else wait_loads<0>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (full) stage(s + R - 1, next);
+    if (!live) return;
     half8 ph[2], plo[2], qh[2], qlo[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -368,7 +396,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 
 template <int MODE, int T>
 void launch_prod(const NsProd& g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((ns_prod_kernel<MODE, T>), dim3((unsigned)(g.tiles * a.batch)), dim3(256), 0, s, g, a, p);
+  hipLaunchKernelGGL((ns_prod_kernel<MODE, T>), dim3((unsigned)((g.whole + g.rest) * a.batch)), dim3(256), 0, s, g, a, p);
 }
 
 template <int T>
@@ -376,7 +404,8 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
   const NsPlan p = make_plan(a.rows, a.cols);
   double* part = (double*)workspace;
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
-  const int parts = std::max(1, std::min(kNormParts, (a.rows + 15) / 16));
+  // workgroups of a matrix: four rows at a time each, ~1 000 in all
+  const int parts = std::max(1, std::min({kNormParts, (a.rows + 3) / 4, (int)std::max<int64_t>(1, 1024 / a.batch)}));
   const dim3 gi((p.mp / 32) * (p.np / 32), (unsigned)a.batch), gn(parts, (unsigned)a.batch);
   if (a.momentum.p) {
     hipLaunchKernelGGL((ns_norm_kernel<T, true>), gn, dim3(256), 0, s, a, part);
@@ -385,7 +414,8 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     hipLaunchKernelGGL((ns_norm_kernel<T, false>), gn, dim3(256), 0, s, a, part);
     hipLaunchKernelGGL((ns_init_kernel<T, false>), gi, dim3(256), 0, s, a, p, parts, part, ws);
   }
-  const int tm = (p.mp + 127) / 128, tn = (p.np + 127) / 128;
+  // tiles of 128: whole ones (tm, tn), and one more where a partial one follows
+  const int tm = p.mp / 128, tn = p.np / 128, pm = p.mp % 128 != 0, pn = p.np % 128 != 0;
   int cur = 0;
   for (int k = 0; k < a.steps; ++k, cur ^= 1) {
     char *xr = ws + p.x[cur], *xc = xr + 2 * p.xplane, *yr = ws + p.x[cur ^ 1], *yc = yr + 2 * p.xplane;
@@ -397,7 +427,8 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.Rp = g.Rq = p.mp;
     g.K = p.np;
     g.ti = g.tj = tm;
-    g.tiles = tm * (tm + 1) / 2;
+    g.whole = tm * (tm + 1) / 2;
+    g.rest = pm * (tm + 1);
     g.Y = g.Z = ws + p.a;
     g.y_lo = g.z_lo = p.aplane;
     g.f = kSa / (kSx * kSx);
@@ -416,7 +447,8 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.q_lo = g.e_lo = p.xplane;
     g.Rq = p.np;
     g.tj = tn;
-    g.tiles = tm * tn;
+    g.whole = tm * tn;
+    g.rest = (tm + pm) * (tn + pn) - tm * tn;
     g.Y = yc;
     g.Z = yr;
     g.y_lo = g.z_lo = p.xplane;

@@ -30,4 +30,10 @@ __device__ __forceinline__ void op_store(void* p, int64_t e, float v) {
   else ((_Float16*)p)[e] = (_Float16)v;
 }
 
+// waits until at most N of this wave's vector loads are outstanding
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+}
+
 }  // namespace lcn
