@@ -152,8 +152,8 @@ struct Int8Gemm {
 };
 
 // A tile of 64 BI tokens x 64 BJ channels, 2 x 2 waves of 32 BI x 32 BJ, 64
-// bytes of K a stage through a ring of R LDS buffers filled by LDS-DMA, R - 1
-// stages in flight.  A stage holds rows of 64 bytes (four 16-byte units); unit c
+// bytes of K a stage through a ring of R LDS buffers filled by LDS-DMA, R - 1 to
+// R stages in flight.  A stage holds rows of 64 bytes (four 16-byte units); unit c
 // of row r sits at c ^ ((r >> 2) & 3), so the 32 rows of a fragment read spread
 // over all banks; the permutation is made by the lane's choice of global
 // address.  The buffers are separate LDS objects, so the compiler adds no waits
@@ -202,65 +202,68 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0;
   const int nk = (int)(g.kp / 64);
-  // stage s has landed (this wave's loads by the wait, the others' by the
-  // barrier) and every wave has read stage s - 1, whose buffer takes s + R - 1
-  auto step = [&](int s, const char* buf, char* next, bool full) {
-    if (full) wait_loads<(R - 2) * L>();
-    else wait_loads<0>();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (full) stage(s + R - 1, next);
+  struct Frag { v4i p[BI], q[BJ]; };
+  auto fetch = [&](const char* buf, int kk, Frag& f) {
+    const int c = ((2 * kk + h) ^ ((l31 >> 2) & 3)) * 16 + l31 * 64;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4i p[BI], q[BJ];
-      const int c = ((2 * kk + h) ^ ((l31 >> 2) & 3)) * 16 + l31 * 64;
+    for (int x = 0; x < BI; ++x) f.p[x] = *(const v4i*)(buf + (wi * BI + x) * 2048 + c);
 #pragma unroll
-      for (int x = 0; x < BI; ++x) p[x] = *(const v4i*)(buf + (wi * BI + x) * 2048 + c);
+    for (int y = 0; y < BJ; ++y) f.q[y] = *(const v4i*)(buf + BI * 4096 + (wj * BJ + y) * 2048 + c);
+  };
+  auto multiply = [&](const Frag& f) {
 #pragma unroll
-      for (int y = 0; y < BJ; ++y) q[y] = *(const v4i*)(buf + BI * 4096 + (wj * BJ + y) * 2048 + c);
+    for (int x = 0; x < BI; ++x)
 #pragma unroll
-      for (int x = 0; x < BI; ++x)
-#pragma unroll
-        for (int y = 0; y < BJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(p[x], q[y], acc[x][y], 0, 0, 0);
+      for (int y = 0; y < BJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.p[x], f.q[y], acc[x][y], 0, 0, 0);
+  };
+  // A stage is two halves of 32 bytes.  Step s multiplies the first, held in f0,
+  // while the second is read, then the second while the next stage's first is
+  // read.  Past the barrier stage s + 1 has landed for every wave, and every wave
+  // holds the rest of stage s in registers: its buffer takes stage s + R.
+  Frag f0, f1;
+  auto step = [&](int s, char* mine, const char* after, bool more, bool load) {
+    fetch(mine, 1, f1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f0);
+    if (more) {
+      if (load) stage_barrier<(R - 2) * L>();
+      else stage_barrier<0>();
+      if (load) stage(s + R, mine);
+      fetch(after, 0, f0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("" ::: "memory");
+    multiply(f1);
   };
   int ks = 0;
-  if (nk >= 2 * R - 1) {
+  if (nk >= 2 * R) {
     stage(0, l0);
     stage(1, l1);
-    if constexpr (R == 4) stage(2, l2);
+    stage(2, l2);
+    if constexpr (R == 4) stage(3, l3);
+    stage_barrier<(R - 1) * L>();
+    fetch(l0, 0, f0);
     do {
-      if constexpr (R == 4) {
-        step(ks, l0, l3, true);
-        step(ks + 1, l1, l0, true);
-        step(ks + 2, l2, l1, true);
-        step(ks + 3, l3, l2, true);
-      } else {
-        step(ks, l0, l2, true);
-        step(ks + 1, l1, l0, true);
-        step(ks + 2, l2, l1, true);
-      }
+      step(ks, l0, l1, true, true);
+      step(ks + 1, l1, l2, true, true);
+      step(ks + 2, l2, R == 4 ? l3 : l0, true, true);
+      if constexpr (R == 4) step(ks + 3, l3, l0, true, true);
       ks += R;
-    } while (ks + 2 * R - 1 <= nk);
+    } while (ks + 2 * R <= nk);
   } else {
     stage(0, l0);
     if (nk > 1) stage(1, l1);
-    if (R == 4 && nk > 2) stage(2, l2);
+    if (nk > 2) stage(2, l2);
+    if (R == 4 && nk > 3) stage(3, l3);
+    stage_barrier<0>();
+    fetch(l0, 0, f0);
   }
-  for (; ks < nk; ks += R) {
+  for (; ks < nk; ks += R) {  // at most 2 R - 1 stages remain
     const int left = nk - ks;
-    if constexpr (R == 4) {
-      step(ks, l0, l3, left > 3);
-      if (left > 1) step(ks + 1, l1, l0, left > 4);
-      if (left > 2) step(ks + 2, l2, l1, left > 5);
-      if (left > 3) step(ks + 3, l3, l2, left > 6);
-    } else {
-      step(ks, l0, l2, left > 2);
-      if (left > 1) step(ks + 1, l1, l0, left > 3);
-      if (left > 2) step(ks + 2, l2, l1, left > 4);
-    }
+    step(ks, l0, l1, left > 1, left > R);
+    if (left > 1) step(ks + 1, l1, l2, left > 2, left > R + 1);
+    if (left > 2) step(ks + 2, l2, R == 4 ? l3 : l0, left > 3, left > R + 2);
+    if constexpr (R == 4)
+      if (left > 3) step(ks + 3, l3, l0, left > 4, false);
   }
 #pragma unroll
   for (int y = 0; y < BJ; ++y) {

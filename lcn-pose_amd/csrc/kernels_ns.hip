@@ -192,7 +192,7 @@ struct NsProd {
 
 // One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 16
 // through a ring of four LDS buffers filled by LDS-DMA (16 KB a stage: hi and
-// lo of both operands), three stages in flight: with one stage in flight a
+// lo of both operands), three to four stages in flight: with one stage in flight a
 // lone workgroup of a CU spent three quarters of its time waiting for the next
 // (46 us for six 1088 x 1088 Gram matrices).  The buffers are four LDS objects, and
 // a stage's object is known at compile time, so the compiler adds no waits of
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
   __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
   // The whole tiles of all matrices come first, then those with fewer than four
-  // row blocks of either operand (whose idle waves return the CU to others).
+  // row blocks of either operand.
   const int nwhole = g.whole * (int)a.batch;
   const bool rest = (int)blockIdx.x >= nwhole;
   const int id = rest ? xcd_remap(blockIdx.x - nwhole, gridDim.x - nwhole) : xcd_remap(blockIdx.x, nwhole);
@@ -237,7 +237,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
-  const bool live = ti * 4 + wi * 2 < nPb && tj * 4 + wj * 2 < nQb;  // any block of this wave's 64 x 64 in range
   // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = 4 row blocks x 1 KB
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
@@ -255,62 +254,76 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
   const int nk = g.K / 16;  // even
-  // stage s: its loads have landed (this wave's by the wait, the others' by the
-  // barrier), every wave has read stage s - 1 -- so its buffer takes stage s + 3
-  auto step = [&](int s, const char* buf, char* next, bool full) {
-    if (full) wait_loads<(R - 2) * L>();
-    else wait_loads<0>();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (full) stage(s + R - 1, next);
-    if (!live) return;
-    half8 ph[2], plo[2], qh[2], qlo[2];
+  struct Frag { half8 ph[2], pl[2], qh[2], ql[2]; };
+  auto fetch = [&](const char* buf, Frag& f) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int op = (wi * 2 + x) * 1024 + vo, oq = (wj * 2 + x) * 1024 + vo;
-      ph[x] = *(const half8*)(buf + op);
-      plo[x] = *(const half8*)(buf + 4096 + op);
-      qh[x] = *(const half8*)(buf + 8192 + oq);
-      qlo[x] = *(const half8*)(buf + 12288 + oq);
+      f.ph[x] = *(const half8*)(buf + op);
+      f.qh[x] = *(const half8*)(buf + 8192 + oq);
+      f.ql[x] = *(const half8*)(buf + 12288 + oq);
+      f.pl[x] = *(const half8*)(buf + 4096 + op);
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], qh[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[x], qlo[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(plo[x], qh[y], acc[x][y], 0, 0, 0);
-    asm volatile("" ::: "memory");
   };
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[x], f.qh[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[x], f.ql[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[x], f.qh[y], acc[x][y], 0, 0, 0);
+  };
+  // Step s multiplies stage s, whose fragments are in `cur`, and reads those of
+  // stage s + 1 meanwhile.  Past the barrier stage s + 1 has landed for every
+  // wave, and every wave holds stage s in registers: its buffer takes stage
+  // s + R.  (Without the fetch ahead a lone workgroup of a CU waits for its LDS
+  // reads before each stage's products.)
+  auto step = [&](int s, char* mine, const char* after, Frag& cur, Frag& next, bool more, bool load) {
+    if (more) {
+      if (load) stage_barrier<(R - 2) * L>();
+      else stage_barrier<0>();
+      if (load) stage(s + R, mine);
+      fetch(after, next);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    multiply(cur);
+  };
+  Frag f0, f1;
   int ks = 0;
-  if (nk >= 2 * R - 1) {  // (a block of its own: the compiler then knows how many loads are outstanding in the loop)
+  if (nk >= 2 * R) {  // (a block of its own: the compiler then knows how many loads are outstanding in the loop)
     stage(0, l0);
     stage(1, l1);
     stage(2, l2);
+    stage(3, l3);
+    stage_barrier<(R - 1) * L>();
+    fetch(l0, f0);
     do {  // every step has a stage left to load
-      step(ks, l0, l3, true);
-      step(ks + 1, l1, l0, true);
-      step(ks + 2, l2, l1, true);
-      step(ks + 3, l3, l2, true);
+      step(ks, l0, l1, f0, f1, true, true);
+      step(ks + 1, l1, l2, f1, f0, true, true);
+      step(ks + 2, l2, l3, f0, f1, true, true);
+      step(ks + 3, l3, l0, f1, f0, true, true);
       ks += R;
-    } while (ks + 2 * R - 1 <= nk);
+    } while (ks + 2 * R <= nk);
   } else {
     stage(0, l0);
     if (nk > 1) stage(1, l1);
     if (nk > 2) stage(2, l2);
+    if (nk > 3) stage(3, l3);
+    stage_barrier<0>();
+    fetch(l0, f0);
   }
-  for (; ks < nk; ks += R) {  // at most six stages remain
+  for (; ks < nk; ks += R) {  // at most seven stages remain
     const int left = nk - ks;
-    step(ks, l0, l3, left > 3);
-    if (left > 1) step(ks + 1, l1, l0, left > 4);
-    if (left > 2) step(ks + 2, l2, l1, left > 5);
-    if (left > 3) step(ks + 3, l3, l2, left > 6);
+    step(ks, l0, l1, f0, f1, left > 1, left > 4);
+    if (left > 1) step(ks + 1, l1, l2, f1, f0, left > 2, left > 5);
+    if (left > 2) step(ks + 2, l2, l3, f0, f1, left > 3, left > 6);
+    if (left > 3) step(ks + 3, l3, l0, f1, f0, left > 4, false);
   }
   __syncthreads();
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own

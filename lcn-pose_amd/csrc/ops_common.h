@@ -30,10 +30,17 @@ __device__ __forceinline__ void op_store(void* p, int64_t e, float v) {
   else ((_Float16*)p)[e] = (_Float16)v;
 }
 
-// waits until at most N of this wave's vector loads are outstanding
+// Waits until at most N of this wave's vector loads are outstanding and all its
+// LDS reads have returned, then for the other waves of the workgroup.  Nothing
+// that touches memory moves across.
 template <int N>
-__device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70);
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
 }
 
 }  // namespace lcn
