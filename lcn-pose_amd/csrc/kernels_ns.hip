@@ -407,26 +407,367 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     }
 }
 
+// ---- matrices with a short side of at most 128 ---------------------------------------------
+// The short side's Gram matrix fits into LDS, so a workgroup does a whole step
+// for its own columns of X: A (from all workgroups' partial sums), B = b A + c A A
+// (every workgroup for itself), X <- a X + B X, and the next Gram matrix's
+// partial sum.  A step is one launch instead of three, and a matrix of few
+// columns is one launch in all.  X is held as chunks of W columns, each an LDS
+// image of Xc and Xr; a workgroup (slab) takes chunks slab, slab + S, ...
+// Bound by latency: launches, barriers and LDS round trips.
+enum { kSolo = 0, kFirst = 1, kMid = 2, kLast = 3 };
+
+struct ThinPlan {
+  int m, n, chunks, slabs;
+  int64_t grams, images, stride;  // per matrix: offsets of the partial sums (two sets) and the images; bytes
+};
+template <int MB, int WB>
+struct ThinGeo {
+  static constexpr int M = 32 * MB, W = 32 * WB;
+  static constexpr int kA = M * M * 2, kX = M * W * 2;     // bytes of a plane of A / B and of X
+  static constexpr int kImage = 4 * kX;                    // Xc hi, Xc lo, Xr hi, Xr lo
+  static constexpr int kLds = kImage + 2 * kA;
+  static constexpr int kGram = M * M * 4;                  // bytes of a partial Gram matrix
+  static constexpr int GB = (MB * MB + 3) / 4, XB = (MB * WB + 3) / 4;  // 32 x 32 blocks a wave holds
+};
+template <int MB, int WB>
+ThinPlan make_thin(int64_t rows, int64_t cols) {
+  using G = ThinGeo<MB, WB>;
+  ThinPlan p;
+  p.m = (int)std::min(rows, cols);
+  p.n = (int)std::max(rows, cols);
+  p.chunks = (p.n + G::W - 1) / G::W;
+  p.slabs = std::min(p.chunks, 48);
+  p.grams = 0;
+  p.images = 2 * (int64_t)p.slabs * G::kGram;
+  p.stride = p.chunks == 1 ? 0 : p.images + (int64_t)p.chunks * G::kImage;
+  return p;
+}
+
+// D += P Q^T for one 32 x 32 block: rows of block rp of plane pair P, rq of Q,
+// contraction length K; both LDS planes with their lo plane `lo` bytes behind
+template <int K>
+__device__ __forceinline__ void lds_product(const char* P, int p_lo, int rp, const char* Q, int q_lo, int rq, int lane,
+                                            f32x16& acc, f32x16& cr) {
+  const char* p = P + rp * (K * 64) + lane * 16;
+  const char* q = Q + rq * (K * 64) + lane * 16;
+#pragma unroll
+  for (int kk = 0; kk < K / 16; ++kk) {
+    const half8 ph = *(const half8*)(p + kk * 1024), pl = *(const half8*)(p + p_lo + kk * 1024);
+    const half8 qh = *(const half8*)(q + kk * 1024), ql = *(const half8*)(q + q_lo + kk * 1024);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    cr = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, cr, 0, 0, 0);
+    cr = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, cr, 0, 0, 0);
+  }
+}
+
+template <int MB, int WB, int T, bool kMuon, int MODE>
+__global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int parts, const double* __restrict__ part,
+                                                      char* __restrict__ ws, int set) {
+  using G = ThinGeo<MB, WB>;
+  constexpr int M = G::M, W = G::W;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char *sc = lds, *sr = lds + 2 * G::kX, *sa = lds + G::kImage;
+  __shared__ double red[4];
+  const int64_t b = blockIdx.y;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, l31 = lane & 31;
+  const bool tall = a.rows > a.cols;
+  char* mine = ws + b * p.stride;
+
+  // the source element of X's (i, j): the gradient, or muon's update direction
+  auto source = [&](int i, int j) {
+    const int64_t r = tall ? j : i, c = tall ? i : j;
+    float v = op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c);
+    if constexpr (kMuon) {
+      const float mo = ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c];
+      v = a.nesterov ? fmaf(a.beta, mo, v) : mo;
+    }
+    return v;
+  };
+  // chunk `ch` of X0 into both LDS forms (zero outside the matrix)
+  auto load_source = [&](int ch, double norm2) {
+    const double inv = (double)kSx / fmax(sqrt(norm2), (double)a.eps);
+    const bool bad = !(norm2 < 1e300);
+    for (int e = threadIdx.x; e < M * W; e += 256) {
+      const int i = tall ? e % M : e / W, j = tall ? e / M : e % W, gj = ch * W + j;
+      float v = 0.f;
+      if (i < p.m && gj < p.n) v = bad ? __builtin_nanf("") : (float)((double)source(i, gj) * inv);
+      _Float16 hi, lo;
+      split(v, hi, lo);
+      char* c = sc + ((((j >> 5) * (M / 8) + (i >> 3)) * 32 + (j & 31)) * 8 + (i & 7)) * 2;
+      char* r = sr + ((((i >> 5) * (W / 8) + (j >> 3)) * 32 + (i & 31)) * 8 + (j & 7)) * 2;
+      *(_Float16*)c = hi;
+      *(_Float16*)(c + G::kX) = lo;
+      *(_Float16*)r = hi;
+      *(_Float16*)(r + G::kX) = lo;
+    }
+  };
+  // one block in (row j, contraction i) form into plane pair `to` of contraction length M
+  auto put = [&](char* to, int lo_at, int bj, int bi, const float (&v)[16]) {
+    char* y = to + ((bj * (M / 8) + bi * 4) * 32 + l31) * 16 + h * 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      half4 hv, lv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 hi, lo;
+        split(v[4 * q + e], hi, lo);
+        hv[e] = hi;
+        lv[e] = lo;
+      }
+      *(half4*)(y + q * 512) = hv;
+      *(half4*)(y + lo_at + q * 512) = lv;
+    }
+  };
+  auto get = [&](const char* from, int lo_at, int bj, int bi, float (&v)[16]) {
+    const char* y = from + ((bj * (M / 8) + bi * 4) * 32 + l31) * 16 + h * 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const half4 hv = *(const half4*)(y + q * 512), lv = *(const half4*)(y + lo_at + q * 512);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = (float)hv[e] + (float)lv[e];
+    }
+  };
+  // this wave's blocks of X X^T of the chunk in LDS, added to g
+  auto gram = [&](f32x16 (&g)[G::GB]) {
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) {
+        f32x16 cr = {};
+        lds_product<W>(sr, G::kX, t % MB, sr, G::kX, t / MB, lane, g[k], cr);
+        g[k] += cr;
+      }
+    }
+  };
+  // A (scaled sums g) into sa, then B = b A + c A A in its place
+  auto square = [&](f32x16 (&g)[G::GB]) {
+    float v[G::GB][16];
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[k][e] = g[k][e] * (kSa / (kSx * kSx));
+        put(sa, G::kA, t / MB, t % MB, v[k]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) {
+        f32x16 acc = {}, cr = {};
+        lds_product<M>(sa, G::kA, t % MB, sa, G::kA, t / MB, lane, acc, cr);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[k][e] = fmaf(acc[e] + cr[e], a.c * kSb / (kSa * kSa), v[k][e] * (a.b * kSb / kSa));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) put(sa, G::kA, t / MB, t % MB, v[k]);
+    }
+    __syncthreads();
+  };
+  // X <- a X + B X for the chunk in LDS; the last step writes the result
+  auto update = [&](int ch, bool last) {
+    float v[G::XB][16];
+    const float sy = last ? 1.f : kSx;
+#pragma unroll
+    for (int k = 0; k < G::XB; ++k) {
+      const int t = w + 4 * k, bi = t % MB, bj = t / MB;
+      if (t < MB * WB) {
+        f32x16 acc = {}, cr = {};
+        lds_product<M>(sa, G::kA, bi, sc, G::kX, bj, lane, acc, cr);
+        get(sc, G::kX, bj, bi, v[k]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[k][e] = fmaf(acc[e] + cr[e], sy / (kSb * kSx), v[k][e] * (a.a * sy / kSx));
+      }
+    }
+    if (last) {
+      const float lr = kMuon ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
+#pragma unroll
+      for (int k = 0; k < G::XB; ++k) {
+        const int t = w + 4 * k, bi = t % MB, j = ch * W + (t / MB) * 32 + l31;
+        if (t >= MB * WB || j >= p.n) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = bi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+          if (i >= p.m) continue;
+          const int64_t o = b * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j);
+          if constexpr (kMuon) {
+            float* P = (float*)a.out.p + o;
+            *P = fmaf(-lr * a.scale, v[k][e], *P * (1.f - lr * a.decay));
+          } else {
+            op_store<T>(a.out.p, o, v[k][e]);
+          }
+        }
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < G::XB; ++k) {
+      const int t = w + 4 * k, bi = t % MB, bj = t / MB;
+      if (t >= MB * WB) continue;
+      put(sc, G::kX, bj, bi, v[k]);
+      // the (row i, contraction j) form, a half at a time
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i31 = 8 * (e >> 2) + 4 * h + (e & 3);
+        _Float16 hi, lo;
+        split(v[k][e], hi, lo);
+        char* r = sr + (((bi * (W / 8) + bj * 4 + (l31 >> 3)) * 32 + i31) * 8 + (l31 & 7)) * 2;
+        *(_Float16*)r = hi;
+        *(_Float16*)(r + G::kX) = lo;
+      }
+    }
+    __syncthreads();
+  };
+
+  f32x16 g[G::GB] = {};
+  if constexpr (MODE == kSolo) {
+    // the norm (and the momentum): every element once, then X0 from the same data
+    double s = 0.0;
+    for (int e = threadIdx.x; e < a.rows * a.cols; e += 256) {
+      const int r = e / a.cols, c = e - r * a.cols;
+      float v = op_load<T>(a.in.p, b * a.in.batch + (int64_t)r * a.in.row + c);
+      if constexpr (kMuon) {
+        float* mo = (float*)a.momentum.p + b * a.momentum.batch + (int64_t)r * a.momentum.row + c;
+        const float m1 = fmaf(a.beta, *mo, v);
+        *mo = m1;
+        v = a.nesterov ? fmaf(a.beta, m1, v) : m1;
+      }
+      s = fma((double)v, (double)v, s);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) red[w] = s;
+    __syncthreads();  // (also orders the momentum written above before its reads below)
+    load_source(0, (red[0] + red[1]) + (red[2] + red[3]));
+    __syncthreads();
+    for (int k = 0; k < a.steps; ++k) {
+#pragma unroll
+      for (int q = 0; q < G::GB; ++q) g[q] = {};
+      gram(g);
+      square(g);
+      update(0, k + 1 == a.steps);
+    }
+    return;
+  }
+
+  const int slab = blockIdx.x;
+  float* gin = (float*)(mine + p.grams + (int64_t)set * p.slabs * G::kGram);
+  float* gout = (float*)(mine + p.grams + (int64_t)(set ^ 1) * p.slabs * G::kGram) + (int64_t)slab * (G::kGram / 4);
+  if constexpr (MODE != kFirst) {
+    // A from the slabs' partial sums, in slab order
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) {
+        for (int q = 0; q < p.slabs; ++q) {
+          const float4* src = (const float4*)(gin + (int64_t)q * (G::kGram / 4) + (t * 64 + lane) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 f = src[e];
+            g[k][4 * e] += f.x; g[k][4 * e + 1] += f.y; g[k][4 * e + 2] += f.z; g[k][4 * e + 3] += f.w;
+          }
+        }
+      }
+    }
+    square(g);
+#pragma unroll
+    for (int q = 0; q < G::GB; ++q) g[q] = {};
+  }
+  const double norm2 = MODE == kFirst ? norm2_of(part + b * kNormParts, parts) : 0.0;
+  for (int ch = slab; ch < p.chunks; ch += p.slabs) {
+    char* image = mine + p.images + (int64_t)ch * G::kImage;
+    __syncthreads();  // the chunk before is done with
+    if constexpr (MODE == kFirst) {
+      load_source(ch, norm2);
+    } else {
+      for (int e = threadIdx.x; e < G::kImage / 16; e += 256)
+        if (MODE != kLast || e < G::kImage / 32) ((v4u*)lds)[e] = ((const v4u*)image)[e];  // (the last step reads Xc only)
+    }
+    __syncthreads();
+    if constexpr (MODE != kFirst) update(ch, MODE == kLast);
+    if constexpr (MODE != kLast) {
+      gram(g);
+      for (int e = threadIdx.x; e < G::kImage / 16; e += 256) ((v4u*)image)[e] = ((const v4u*)lds)[e];
+    }
+  }
+  if constexpr (MODE != kLast) {
+#pragma unroll
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + 4 * k;
+      if (t < MB * MB) {
+        float4* dst = (float4*)(gout + (t * 64 + lane) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[e] = make_float4(g[k][4 * e], g[k][4 * e + 1], g[k][4 * e + 2], g[k][4 * e + 3]);
+      }
+    }
+  }
+}
+
+template <int T, bool kMuon>
+void launch_norm(const NsArgs& a, int parts, double* part, hipStream_t s) {
+  hipLaunchKernelGGL((ns_norm_kernel<T, kMuon>), dim3(parts, (unsigned)a.batch), dim3(256), 0, s, a, part);
+}
+// workgroups of the norm for a matrix: four rows at a time each, ~1 000 in all
+int norm_parts(const NsArgs& a) {
+  return std::max(1, std::min({kNormParts, (a.rows + 3) / 4, (int)std::max<int64_t>(1, 1024 / a.batch)}));
+}
+
+template <int MB, int WB, int T, bool kMuon>
+void launch_thin(const NsArgs& a, void* workspace, hipStream_t s) {
+  using G = ThinGeo<MB, WB>;
+  const ThinPlan p = make_thin<MB, WB>(a.rows, a.cols);
+  double* part = (double*)workspace;
+  char* ws = (char*)workspace + a.batch * kNormParts * 8;
+  if (p.chunks == 1) {
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kSolo>), dim3(1, (unsigned)a.batch), dim3(256), G::kLds, s, a, p, 0, part, ws, 0);
+    return;
+  }
+  const dim3 grid(p.slabs, (unsigned)a.batch);
+  const int parts = norm_parts(a);
+  launch_norm<T, kMuon>(a, parts, part, s);
+  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kFirst>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, 1);
+  int set = 0;
+  for (int k = 0; k + 1 < a.steps; ++k, set ^= 1)
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kMid>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, set);
+  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kLast>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, set);
+}
+
+// The path of a matrix by its sides: short side at most 64 with chunks of 64
+// columns where one holds the long side, else of 128; at most 128 with chunks of
+// 64; larger ones in tiles.
+enum { kThinSmall, kThin64, kThin128, kTiled };
+int path_of(int64_t rows, int64_t cols) {
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  if (m <= 64) return n <= 64 ? kThinSmall : kThin64;
+  return m <= 128 ? kThin128 : kTiled;
+}
+
 template <int MODE, int T>
 void launch_prod(const NsProd& g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((ns_prod_kernel<MODE, T>), dim3((unsigned)((g.whole + g.rest) * a.batch)), dim3(256), 0, s, g, a, p);
 }
 
-template <int T>
+template <int T, bool kMuon>
 void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
+  switch (path_of(a.rows, a.cols)) {
+    case kThinSmall: return launch_thin<2, 2, T, kMuon>(a, workspace, s);
+    case kThin64: return launch_thin<2, 4, T, kMuon>(a, workspace, s);
+    case kThin128: return launch_thin<4, 2, T, kMuon>(a, workspace, s);
+  }
   const NsPlan p = make_plan(a.rows, a.cols);
   double* part = (double*)workspace;
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
-  // workgroups of a matrix: four rows at a time each, ~1 000 in all
-  const int parts = std::max(1, std::min({kNormParts, (a.rows + 3) / 4, (int)std::max<int64_t>(1, 1024 / a.batch)}));
-  const dim3 gi((p.mp / 32) * (p.np / 32), (unsigned)a.batch), gn(parts, (unsigned)a.batch);
-  if (a.momentum.p) {
-    hipLaunchKernelGGL((ns_norm_kernel<T, true>), gn, dim3(256), 0, s, a, part);
-    hipLaunchKernelGGL((ns_init_kernel<T, true>), gi, dim3(256), 0, s, a, p, parts, part, ws);
-  } else {
-    hipLaunchKernelGGL((ns_norm_kernel<T, false>), gn, dim3(256), 0, s, a, part);
-    hipLaunchKernelGGL((ns_init_kernel<T, false>), gi, dim3(256), 0, s, a, p, parts, part, ws);
-  }
+  const int parts = norm_parts(a);
+  launch_norm<T, kMuon>(a, parts, part, s);
+  hipLaunchKernelGGL((ns_init_kernel<T, kMuon>), dim3((p.mp / 32) * (p.np / 32), (unsigned)a.batch), dim3(256), 0, s, a, p, parts, part, ws);
   // tiles of 128: whole ones (tm, tn), and one more where a partial one follows
   const int tm = p.mp / 128, tn = p.np / 128, pm = p.mp % 128 != 0, pn = p.np % 128 != 0;
   int cur = 0;
@@ -478,14 +819,29 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
 
 int64_t ns_workspace(int64_t batch, int64_t rows, int64_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  return batch * (kNormParts * 8 + make_plan(rows, cols).stride);
+  int64_t stride = 0;
+  switch (path_of(rows, cols)) {
+    case kThinSmall: stride = make_thin<2, 2>(rows, cols).stride; break;
+    case kThin64: stride = make_thin<2, 4>(rows, cols).stride; break;
+    case kThin128: stride = make_thin<4, 2>(rows, cols).stride; break;
+    default: stride = make_plan(rows, cols).stride;
+  }
+  return batch * (kNormParts * 8 + stride);
 }
+
+namespace {
+template <int T>
+void launch_by_kind(const NsArgs& a, void* workspace, hipStream_t s) {
+  if (a.momentum.p) launch_ns_t<T, true>(a, workspace, s);
+  else launch_ns_t<T, false>(a, workspace, s);
+}
+}  // namespace
 
 void launch_ns(const NsArgs& a, void* workspace, hipStream_t s) {
   // T: the type read (and, by orthogonalize, written); the parameter of muon is fp32
-  if (a.dtype == kOpF32) launch_ns_t<kOpF32>(a, workspace, s);
-  else if (a.dtype == kOpBF16) launch_ns_t<kOpBF16>(a, workspace, s);
-  else launch_ns_t<kOpF16>(a, workspace, s);
+  if (a.dtype == kOpF32) launch_by_kind<kOpF32>(a, workspace, s);
+  else if (a.dtype == kOpBF16) launch_by_kind<kOpBF16>(a, workspace, s);
+  else launch_by_kind<kOpF16>(a, workspace, s);
 }
 
 }  // namespace lcn

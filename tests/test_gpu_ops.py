@@ -58,7 +58,7 @@ def gradient(shape, dtype, seed=0):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (5, 5), (17, 34), (31, 33), (32, 32), (33, 31), (51, 1088), (63, 64), (64, 64), (65, 64),
-          (64, 200), (127, 129), (128, 128), (129, 127), (160, 96), (257, 300), (300, 257)]
+          (64, 200), (127, 129), (128, 128), (129, 127), (160, 96), (257, 300), (300, 257), (1, 300), (40, 7001), (6500, 20), (97, 128), (128, 65), (100, 4001), (4001, 70)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -145,7 +145,7 @@ def test_orthogonalize_repeats_bitwise():
 
 def test_orthogonalize_stays_inside_its_workspace():
     lib = native.load_library()
-    for shape in ((2, 70, 300), (3, 64, 64), (1, 300, 70), (1, 1, 1), (4, 33, 95)):
+    for shape in ((2, 70, 300), (3, 64, 64), (1, 300, 70), (1, 1, 1), (4, 33, 95), (2, 200, 140), (1, 40, 6400)):
         g = gradient(shape, torch.float32)
         out = torch.empty_like(g)
         need = lib.lcn_orthogonalize_workspace(*shape)
