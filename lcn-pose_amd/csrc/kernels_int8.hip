@@ -194,6 +194,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
 #pragma unroll
     for (int i = 0; i < BJ; ++i) I8_LDS(rw, vow[i], so, d + (BI + i) * 4096);
   };
+  __shared__ float qs[64 * BI];  // the tokens' scales
+  if (threadIdx.x < trows) qs[threadIdx.x] = g.qs[t0 + threadIdx.x];
   v16i acc[BI][BJ];
 #pragma unroll
   for (int x = 0; x < BI; ++x)
@@ -265,22 +267,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
     if constexpr (R == 4)
       if (left > 3) step(ks + 3, l3, l0, left > 4, false);
   }
+  const int rows = trows - wi * BI * 32;  // of this wave
 #pragma unroll
   for (int y = 0; y < BJ; ++y) {
     const int n = n0 + (wj * BJ + y) * 32 + l31;
-    if (n >= g.n) continue;
-    const float sw = g.ws[n], b = g.bias ? g.bias[n] : 0.f;
+    const bool in = n < g.n;
+    const float sw = in ? g.ws[n] : 0.f, b = in && g.bias ? g.bias[n] : 0.f;
 #pragma unroll
     for (int x = 0; x < BI; ++x)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int64_t t = t0 + (wi * BI + x) * 32 + 8 * q + 4 * h;
+        const int r = x * 32 + 8 * q + 4 * h;
+        const float4 s4 = *(const float4*)(qs + wi * BI * 32 + r);
+        const float se[4] = {s4.x, s4.y, s4.z, s4.w};
+        const int64_t o = (t0 + wi * BI * 32 + r) * g.out_row + n;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (t + e >= g.tokens) continue;
-          float v = (float)acc[x][y][4 * q + e] * g.qs[t + e] * sw;
+          float v = (float)acc[x][y][4 * q + e] * se[e] * sw;
           if (g.bias) v += b;
-          op_store<T>(g.out, (t + e) * g.out_row + n, v);
+          if (in && r + e < rows) op_store<T>(g.out, o + e * g.out_row, v);
         }
       }
   }

@@ -179,7 +179,7 @@ struct NsProd {
   int64_t p_lo, q_lo;
   int Rp, Rq, K;                      // rows (multiples of 32) of P and Q, contraction length
   int64_t stride;                     // bytes between the matrices' workspaces
-  int ti, tj;                         // 128-row tiles of P and Q that are whole
+  int ti, tj;                         // tiles of P and Q that are whole
   int whole, rest;                    // tiles of a matrix: whole ones, ones with a partial row block
   const char* E; int64_t e_lo;        // kSquare: A (= Q); kUpdate / kFinal: Xc, in (row j, contraction i) form
   char* Y; int64_t y_lo;              // result in (row j, contraction i) form
@@ -190,19 +190,21 @@ struct NsProd {
 #define NS_LDS(SRC, VOFF, SOFF, DST) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
 
-// One 128 x 128 tile of D = P Q^T, four waves of 64 x 64; K in steps of 16
-// through a ring of four LDS buffers filled by LDS-DMA (16 KB a stage: hi and
-// lo of both operands), three to four stages in flight: with one stage in flight a
+// One tile of D = P Q^T with sides of 64 NB, four waves of 32 NB x 32 NB blocks;
+// K in steps of 16 (NB 2) or 32 (NB 1) through a ring of four LDS buffers filled
+// by LDS-DMA (16 KB a stage: hi and lo of both operands), three to four stages
+// in flight: with one stage in flight a
 // lone workgroup of a CU spent three quarters of its time waiting for the next
 // (46 us for six 1088 x 1088 Gram matrices).  The buffers are four LDS objects, and
 // a stage's object is known at compile time, so the compiler adds no waits of
 // its own for loads into the others.
-template <int MODE, int T>
+template <int MODE, int T, int NB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void ns_prod_kernel(NsProd g, NsArgs a, NsPlan pl) {
   constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
+  constexpr int KK = 2 / NB, TB = 2 * NB;  // 16-wide pieces of K a stage, row blocks of a tile's side
   __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
-  // The whole tiles of all matrices come first, then those with fewer than four
-  // row blocks of either operand.
+  // The whole tiles of all matrices come first, then those with fewer row blocks
+  // of either operand.
   const int nwhole = g.whole * (int)a.batch;
   const bool rest = (int)blockIdx.x >= nwhole;
   const int id = rest ? xcd_remap(blockIdx.x - nwhole, gridDim.x - nwhole) : xcd_remap(blockIdx.x, nwhole);
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     ti = t % g.ti;
     tj = t / g.ti;
   } else {  // the last column of tiles, if partial, then the last row
-    const int side = g.Rq / 32 > g.tj * 4 ? g.ti : 0;
+    const int side = g.Rq / 32 > g.tj * TB ? g.ti : 0;
     ti = t < side ? t : g.ti;
     tj = t < side ? g.tj : t - side;
   }
@@ -228,56 +230,61 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const char* Pm = g.P + mat * g.stride;
   const char* Qm = g.Q + mat * g.stride;
   const int nPb = g.Rp / 32, nQb = g.Rq / 32;
-  // this wave stages row block w of both operand tiles (a block past the end
-  // repeats the last one; its results are not stored)
+  // this wave stages one row block (NB 1: one 16-wide piece of it) of both operand
+  // tiles (a block past the end repeats the last one; its results are not stored)
+  const int sb = NB == 2 ? w : w >> 1, sk = NB == 2 ? 0 : (w & 1) * 1024;
   const int rb_bytes = g.K * 64;
-  const int pb = min(ti * 4 + w, nPb - 1), qb = min(tj * 4 + w, nQb - 1);
+  const int pb = min(ti * TB + sb, nPb - 1), qb = min(tj * TB + sb, nQb - 1);
   const __amdgpu_buffer_rsrc_t rph = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rpl = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + g.p_lo + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
-  // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = 4 row blocks x 1 KB
+  // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = row blocks x 1 KB pieces of K
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
-    const int so = ks * 1024;
+    const int so = ks * (1024 * KK) + sk;
     NS_LDS(rph, vo, so, d);
     NS_LDS(rpl, vo, so, d + 4096);
     NS_LDS(rqh, vo, so, d + 8192);
     NS_LDS(rql, vo, so, d + 12288);
   };
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
-  const int nk = g.K / 16;  // even
-  struct Frag { half8 ph[2], pl[2], qh[2], ql[2]; };
+  f32x16 acc[NB][NB] = {}, cr = {};  // cr: NB 1 alternates between two sums, which do not wait for each other
+  const int nk = g.K / (16 * KK);
+  struct Frag { half8 ph[NB * KK], pl[NB * KK], qh[NB * KK], ql[NB * KK]; };  // [row block][piece of K]
   auto fetch = [&](const char* buf, Frag& f) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int op = (wi * 2 + x) * 1024 + vo, oq = (wj * 2 + x) * 1024 + vo;
+    for (int x = 0; x < NB * KK; ++x) {
+      const int op = (wi * NB * KK + x) * 1024 + vo, oq = (wj * NB * KK + x) * 1024 + vo;
       f.ph[x] = *(const half8*)(buf + op);
       f.qh[x] = *(const half8*)(buf + 8192 + oq);
       f.ql[x] = *(const half8*)(buf + 12288 + oq);
       f.pl[x] = *(const half8*)(buf + 4096 + op);
     }
   };
+#define NS_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_f16(A, B, C, 0, 0, 0)
   auto multiply = [&](const Frag& f) {
+    if constexpr (NB == 1) {
+      acc[0][0] = NS_MFMA(f.ph[0], f.qh[0], acc[0][0]);
+      cr = NS_MFMA(f.ph[0], f.ql[0], cr);
+      acc[0][0] = NS_MFMA(f.pl[0], f.qh[0], acc[0][0]);
+      cr = NS_MFMA(f.ph[1], f.qh[1], cr);
+      acc[0][0] = NS_MFMA(f.ph[1], f.ql[1], acc[0][0]);
+      cr = NS_MFMA(f.pl[1], f.qh[1], cr);
+    } else {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < NB; ++x)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[x], f.qh[y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.qh[y], acc[x][y]);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < NB; ++x)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[x], f.ql[y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.ql[y], acc[x][y]);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < NB; ++x)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[x], f.qh[y], acc[x][y], 0, 0, 0);
+        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.pl[x], f.qh[y], acc[x][y]);
+    }
   };
   // Step s multiplies stage s, whose fragments are in `cur`, and reads those of
   // stage s + 1 meanwhile.  Past the barrier stage s + 1 has landed for every
@@ -325,15 +332,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     if (left > 2) step(ks + 2, l2, l3, f0, f1, left > 3, left > 6);
     if (left > 3) step(ks + 3, l3, l0, f1, f0, left > 4, false);
   }
+  if constexpr (NB == 1) acc[0][0] += cr;
   __syncthreads();
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
   unsigned* tr = (unsigned*)(w == 0 ? l0 : w == 1 ? l1 : w == 2 ? l2 : l3);
   const float lr = MODE == kFinal && a.momentum.p ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < NB; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int rbi = ti * 4 + wi * 2 + x, rbj = tj * 4 + wj * 2 + y;
+    for (int y = 0; y < NB; ++y) {
+      const int rbi = ti * TB + wi * NB + x, rbj = tj * TB + wj * NB + y;
       if (rbi >= nPb || rbj >= nQb) continue;
       float v[16];
 #pragma unroll
@@ -488,10 +496,11 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
   auto load_source = [&](int ch, double norm2) {
     const double inv = (double)kSx / fmax(sqrt(norm2), (double)a.eps);
     const bool bad = !(norm2 < 1e300);
+#pragma unroll 8
     for (int e = threadIdx.x; e < M * W; e += 256) {
       const int i = tall ? e % M : e / W, j = tall ? e / M : e % W, gj = ch * W + j;
-      float v = 0.f;
-      if (i < p.m && gj < p.n) v = bad ? __builtin_nanf("") : (float)((double)source(i, gj) * inv);
+      float v = i < p.m && gj < p.n ? source(i, gj) : 0.f;
+      v = bad ? __builtin_nanf("") : (float)((double)v * inv);
       _Float16 hi, lo;
       split(v, hi, lo);
       char* c = sc + ((((j >> 5) * (M / 8) + (i >> 3)) * 32 + (j & 31)) * 8 + (i & 7)) * 2;
@@ -661,19 +670,34 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
   const int slab = blockIdx.x;
   float* gin = (float*)(mine + p.grams + (int64_t)set * p.slabs * G::kGram);
   float* gout = (float*)(mine + p.grams + (int64_t)(set ^ 1) * p.slabs * G::kGram) + (int64_t)slab * (G::kGram / 4);
+  // a chunk's image into LDS, by LDS-DMA (the last step reads Xc only)
+  constexpr int kBytes = MODE == kLast ? G::kImage / 2 : G::kImage;
+  auto load_image = [&](int ch) {
+    const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc((void*)(mine + p.images + (int64_t)ch * G::kImage), 0, kBytes, 0x00020000);
+#pragma unroll
+    for (int e = 0; e < kBytes; e += 4096) NS_LDS(res, lane * 16, e + w * 1024, lds + e + w * 1024);
+  };
   if constexpr (MODE != kFirst) {
-    // A from the slabs' partial sums, in slab order
+    load_image(slab);  // meanwhile: A from the slabs' partial sums, in slab order
 #pragma unroll
     for (int k = 0; k < G::GB; ++k) {
       const int t = w + 4 * k;
       if (t < MB * MB) {
-        for (int q = 0; q < p.slabs; ++q) {
-          const float4* src = (const float4*)(gin + (int64_t)q * (G::kGram / 4) + (t * 64 + lane) * 16);
+        const float4* src = (const float4*)(gin + (t * 64 + lane) * 16);
+        constexpr int kAhead = 6, kPitch = G::kGram / 16;  // sums in flight
+        for (int q0 = 0; q0 < p.slabs; q0 += kAhead) {
+          float4 f[kAhead][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 f = src[e];
-            g[k][4 * e] += f.x; g[k][4 * e + 1] += f.y; g[k][4 * e + 2] += f.z; g[k][4 * e + 3] += f.w;
-          }
+          for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              f[q][e] = q0 + q < p.slabs ? src[(int64_t)(q0 + q) * kPitch + e] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              g[k][4 * e] += f[q][e].x; g[k][4 * e + 1] += f[q][e].y; g[k][4 * e + 2] += f[q][e].z; g[k][4 * e + 3] += f[q][e].w;
+            }
         }
       }
     }
@@ -684,13 +708,11 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
   const double norm2 = MODE == kFirst ? norm2_of(part + b * kNormParts, parts) : 0.0;
   for (int ch = slab; ch < p.chunks; ch += p.slabs) {
     char* image = mine + p.images + (int64_t)ch * G::kImage;
-    __syncthreads();  // the chunk before is done with
-    if constexpr (MODE == kFirst) {
-      load_source(ch, norm2);
-    } else {
-      for (int e = threadIdx.x; e < G::kImage / 16; e += 256)
-        if (MODE != kLast || e < G::kImage / 32) ((v4u*)lds)[e] = ((const v4u*)image)[e];  // (the last step reads Xc only)
+    if (ch != slab) {
+      __syncthreads();  // the chunk before is done with
+      if constexpr (MODE != kFirst) load_image(ch);
     }
+    if constexpr (MODE == kFirst) load_source(ch, norm2);
     __syncthreads();
     if constexpr (MODE != kFirst) update(ch, MODE == kLast);
     if constexpr (MODE != kLast) {
@@ -750,9 +772,33 @@ int path_of(int64_t rows, int64_t cols) {
   return m <= 128 ? kThin128 : kTiled;
 }
 
+// Tiles of 128 or 64.  A launch lasts as long as its fullest CU: that many tiles,
+// a tile of 64 a quarter of one of 128 times 1.3 (its operands are read from LDS
+// for half as many products).  Measured, 128 / 64: six 1088 Gram matrices (270
+// tiles of 128) 41 / 33 us, their update (486) 54 / 62; one 1088 Gram (45) 23 / 11,
+// its update (81) 26 / 16; 2000 Gram (136) 44 / 42, its update (256) 54 / 76.
 template <int MODE, int T>
-void launch_prod(const NsProd& g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((ns_prod_kernel<MODE, T>), dim3((unsigned)((g.whole + g.rest) * a.batch)), dim3(256), 0, s, g, a, p);
+void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
+  auto tiles = [&](int side) {  // whole tiles, and one more a side where a partial one follows
+    const int tm = g.Rp / side, tn = g.Rq / side, pm = g.Rp % side != 0, pn = g.Rq % side != 0;
+    g.ti = tm;
+    g.tj = tn;
+    if (MODE == kGram || MODE == kSquare) {
+      g.whole = tm * (tm + 1) / 2;
+      g.rest = pm * (tm + 1);
+    } else {
+      g.whole = tm * tn;
+      g.rest = (tm + pm) * (tn + pn) - tm * tn;
+    }
+    return (g.whole + g.rest) * a.batch;
+  };
+  const int64_t n64 = tiles(64), n = tiles(128);
+  if (13 * ((n64 + 255) / 256) < 40 * ((n + 255) / 256)) {
+    tiles(64);
+    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 1>), dim3((unsigned)n64), dim3(256), 0, s, g, a, p);
+  } else {
+    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 2>), dim3((unsigned)n), dim3(256), 0, s, g, a, p);
+  }
 }
 
 template <int T, bool kMuon>
@@ -768,8 +814,6 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
   const int parts = norm_parts(a);
   launch_norm<T, kMuon>(a, parts, part, s);
   hipLaunchKernelGGL((ns_init_kernel<T, kMuon>), dim3((p.mp / 32) * (p.np / 32), (unsigned)a.batch), dim3(256), 0, s, a, p, parts, part, ws);
-  // tiles of 128: whole ones (tm, tn), and one more where a partial one follows
-  const int tm = p.mp / 128, tn = p.np / 128, pm = p.mp % 128 != 0, pn = p.np % 128 != 0;
   int cur = 0;
   for (int k = 0; k < a.steps; ++k, cur ^= 1) {
     char *xr = ws + p.x[cur], *xc = xr + 2 * p.xplane, *yr = ws + p.x[cur ^ 1], *yc = yr + 2 * p.xplane;
@@ -780,9 +824,6 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.p_lo = g.q_lo = p.xplane;
     g.Rp = g.Rq = p.mp;
     g.K = p.np;
-    g.ti = g.tj = tm;
-    g.whole = tm * (tm + 1) / 2;
-    g.rest = pm * (tm + 1);
     g.Y = g.Z = ws + p.a;
     g.y_lo = g.z_lo = p.aplane;
     g.f = kSa / (kSx * kSx);
@@ -800,9 +841,6 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.Q = g.E = xc;
     g.q_lo = g.e_lo = p.xplane;
     g.Rq = p.np;
-    g.tj = tn;
-    g.whole = tm * tn;
-    g.rest = (tm + pm) * (tn + pn) - tm * tn;
     g.Y = yc;
     g.Z = yr;
     g.y_lo = g.z_lo = p.xplane;
