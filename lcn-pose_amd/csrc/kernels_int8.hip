@@ -7,6 +7,12 @@
 // A row whose largest magnitude is below 2^-100 counts as zero (127 / max would
 // overflow); a row that holds an infinity or a NaN gives NaN throughout: its
 // scale is NaN and its integers are zero.  The sums are exact (int32, K <= 131072).
+//
+// Quantised tokens are stored in panels of 64 of K: element (t, k) at
+// (k / 64) rows 64 + 64 t + k % 64, K padded with zeros.  A panel's rows follow
+// each other, so an LDS-DMA of 16 rows x 64 bytes reads 1 KB of whole cache lines
+// (from row-major integers it reads half of 16 lines: 65 536 x 1088 x 1088 spent
+// 100 of 220 us on that).  Weights that many tiles read are laid out the same way.
 #include <algorithm>
 
 #include "ops_common.h"
@@ -18,6 +24,7 @@ namespace {
 __host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 256; }
 
+constexpr int64_t kPanelTokens = 1024;
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
 
 // the factor 127 / top of a row and its scale, from the largest magnitude
@@ -70,7 +77,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
   float top = 0.f, factor, s;
   bool bad = false;
   const int64_t r = t * x_row;
-  int8_t* out = q + t * kp;
+  int8_t* out = q + t * 64;
+  const int64_t panel = tokens * 64;
   if constexpr (kAligned) {
     constexpr int V = kVec<T>, kRegs = 6;
     const int pieces = k / V;  // k is a multiple of V here
@@ -102,8 +110,9 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[d] |= (bad ? 0u : (unsigned)(quant(v[4 * d + e], factor) & 255)) << (8 * e);
       }
-      if constexpr (V == 4) *(unsigned*)(out + (int64_t)c * 4) = w[0];
-      else *(uint2*)(out + (int64_t)c * 8) = make_uint2(w[0], w[1]);
+      int8_t* o = out + (c * V >> 6) * panel + (c * V & 63);
+      if constexpr (V == 4) *(unsigned*)o = w[0];
+      else *(uint2*)o = make_uint2(w[0], w[1]);
     };
     const int padded = (int)(kp / V);  // the pieces past k hold zeros
 #pragma unroll
@@ -126,25 +135,38 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
     row_scale(top, bad, factor, s);
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
-      if (lane + 64 * i < kp) out[lane + 64 * i] = bad ? (int8_t)0 : (int8_t)quant(keep[i], factor);
-    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[c] = c < k && !bad ? (int8_t)quant(op_load<T>(x, r + c), factor) : (int8_t)0;
+      if (64 * i < kp) out[i * panel + lane] = bad ? (int8_t)0 : (int8_t)quant(keep[i], factor);
+    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[(c >> 6) * panel + lane] = c < k && !bad ? (int8_t)quant(op_load<T>(x, r + c), factor) : (int8_t)0;
   }
   if (lane == 0) scale[t] = s;
 }
 
-// weight rows of any alignment -> rows of kp bytes, zero padded
-__global__ __launch_bounds__(256) void repack_kernel(const int8_t* __restrict__ w, int64_t w_row, int k, int64_t kp,
-                                                     int8_t* __restrict__ out) {
-  const int64_t n = blockIdx.x;
-  for (int64_t c = threadIdx.x; c < kp; c += 256) out[n * kp + c] = c < k ? w[n * w_row + c] : (int8_t)0;
+// weight rows of any alignment -> panels of 64 of K, zero padded; kAligned: rows of
+// whole 4-byte pieces
+template <bool kAligned>
+__global__ __launch_bounds__(256) void panels_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int8_t* __restrict__ out) {
+  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // channel
+  if (c >= n) return;
+  const int k0 = blockIdx.y * 64 + (threadIdx.x & 15) * 4;
+  const int8_t* src = w + c * w_row + k0;
+  unsigned v = 0;
+  if constexpr (kAligned) {
+    if (k0 < k) v = *(const unsigned*)src;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k0 + e < k) v |= (unsigned)(uint8_t)src[e] << (8 * e);
+  }
+  *(unsigned*)(out + ((int64_t)blockIdx.y * n + c) * 64 + (threadIdx.x & 15) * 4) = v;
 }
 
 #define I8_LDS(SRC, VOFF, SOFF, DST) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
 
 struct Int8Gemm {
-  const int8_t* q; const float* qs; int64_t kp;    // [tokens][kp], [tokens]
-  const int8_t* w; int64_t w_row, kw;              // rows of kw bytes (a multiple of 4), 16-byte aligned
+  const int8_t* q; const float* qs; int64_t kp;    // panels of the tokens, their scales, padded K
+  const int8_t* w; int64_t w_row, w_panel;         // 64-byte piece p of row c at p w_panel + c w_row, 16-byte aligned
+  int64_t w_bytes;                                 // readable from w
   const float* ws; const float* bias;
   void* out; int64_t out_row;
   int64_t tokens; int n;
@@ -171,15 +193,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
   const int wi = w >> 1, wj = w & 1, h = lane >> 5, l31 = lane & 31;
   // rows past the end repeat the last one; their results are not stored
   const int trows = (int)min((int64_t)(64 * BI), g.tokens - t0), nrows = min(64 * BJ, g.n - n0);
-  const int64_t qbytes = (int64_t)trows * g.kp, wbytes = (int64_t)(nrows - 1) * g.w_row + g.kw;
-  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(g.q + t0 * g.kp), 0, (int)qbytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + n0 * g.w_row), 0, (int)wbytes, 0x00020000);
+  const int64_t wat = (int64_t)n0 * g.w_row;
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(g.q + t0 * 64), 0, (int)(g.kp * g.tokens - t0 * 64), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + wat), 0, (int)(g.w_bytes - wat), 0x00020000);
+  const int qp = (int)g.tokens * 64, wp = (int)g.w_panel;
   // load i of a wave: 16 rows x 64 bytes
   int voq[BI], vow[BJ];
 #pragma unroll
   for (int i = 0; i < BI; ++i) {
     const int r = (i * 4 + w) * 16 + (lane >> 2);
-    voq[i] = min(r, trows - 1) * (int)g.kp + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
+    voq[i] = min(r, trows - 1) * 64 + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
   }
 #pragma unroll
   for (int i = 0; i < BJ; ++i) {
@@ -188,11 +211,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
   }
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
-    const int so = ks * 64;
+    const int sq = ks * qp, sw = ks * wp;
 #pragma unroll
-    for (int i = 0; i < BI; ++i) I8_LDS(rq, voq[i], so, d + i * 4096);
+    for (int i = 0; i < BI; ++i) I8_LDS(rq, voq[i], sq, d + i * 4096);
 #pragma unroll
-    for (int i = 0; i < BJ; ++i) I8_LDS(rw, vow[i], so, d + (BI + i) * 4096);
+    for (int i = 0; i < BJ; ++i) I8_LDS(rw, vow[i], sw, d + (BI + i) * 4096);
   };
   __shared__ float qs[64 * BI];  // the tokens' scales
   if (threadIdx.x < trows) qs[threadIdx.x] = g.qs[t0 + threadIdx.x];
@@ -267,25 +290,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
     if constexpr (R == 4)
       if (left > 3) step(ks + 3, l3, l0, left > 4, false);
   }
-  const int rows = trows - wi * BI * 32;  // of this wave
+  // The tile of the output as a buffer: its rows end with the tile, so stores of
+  // rows past the tokens are dropped, and lanes past the channels point behind it.
+  // Row offsets are scalar: a store costs no address arithmetic.
+  constexpr int kOut = T == kOpF32 ? 4 : 2;
+  const int64_t obytes = ((int64_t)(trows - 1) * g.out_row + nrows) * kOut;
+  const bool near = obytes < 0x7fffffff;
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((char*)g.out + (t0 * g.out_row + n0) * kOut, 0, (int)obytes, 0x00020000);
 #pragma unroll
   for (int y = 0; y < BJ; ++y) {
-    const int n = n0 + (wj * BJ + y) * 32 + l31;
-    const bool in = n < g.n;
-    const float sw = in ? g.ws[n] : 0.f, b = in && g.bias ? g.bias[n] : 0.f;
+    const int c = (wj * BJ + y) * 32 + l31;
+    const bool in = c < nrows;
+    const float sw = in ? g.ws[n0 + c] : 0.f, b = in && g.bias ? g.bias[n0 + c] : 0.f;
+    const int vout = in ? (4 * h * (int)g.out_row + c) * kOut : -1;
 #pragma unroll
     for (int x = 0; x < BI; ++x)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int r = x * 32 + 8 * q + 4 * h;
-        const float4 s4 = *(const float4*)(qs + wi * BI * 32 + r);
+        const int r = (wi * BI + x) * 32 + 8 * q;
+        const float4 s4 = *(const float4*)(qs + r + 4 * h);
         const float se[4] = {s4.x, s4.y, s4.z, s4.w};
-        const int64_t o = (t0 + wi * BI * 32 + r) * g.out_row + n;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float v = (float)acc[x][y][4 * q + e] * se[e] * sw;
           if (g.bias) v += b;
-          if (in && r + e < rows) op_store<T>(g.out, o + e * g.out_row, v);
+          if (near) {
+            const int so = (r + e) * (int)g.out_row * kOut;
+            if constexpr (T == kOpF32) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), ro, vout, so, 0);
+            else if constexpr (T == kOpBF16) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), ro, vout, so, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (_Float16)v), ro, vout, so, 0);
+          } else if (in && r + 4 * h + e < trows) {
+            op_store<T>(g.out, (t0 + r + 4 * h + e) * g.out_row + n0 + c, v);
+          }
         }
       }
   }
@@ -355,7 +391,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
       if (p >= nk) break;
       v4i q;
       if constexpr (kFused) q = *(const v4i*)(lds + tr * pitch + p * 64 + kq * 16);
-      else q = *(const v4i*)(g.q + (int64_t)tr * kp + p * 64 + kq * 16);
+      else q = *(const v4i*)(g.q + ((int64_t)p * tokens + tr) * 64 + kq * 16);
       const v4i ww = wv[i];
       if (p + 4 * kAhead < nk) wv[i] = weights(p + 4 * kAhead);
       acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q, ww, acc, 0, 0, 0);
@@ -412,18 +448,23 @@ void launch_tiles(Int8Gemm& g, hipStream_t s) {
   hipLaunchKernelGGL((int8_gemm_kernel<T, BI, BJ, R>), dim3((unsigned)(tt * g.tn)), dim3(256), 0, s, g);
 }
 
+// Tokens of one quantise + multiply round: their integers stay below 1 GiB, which
+// 32-bit offsets reach.
+int64_t round_tokens(int64_t tokens, int64_t k) { return std::min(tokens, std::max<int64_t>(256, ((int64_t)1 << 30) / pad64(k) / 256 * 256)); }
+
 template <int T>
-void launch_int8_t(const Int8Args& a, void* workspace, hipStream_t s) {
-  const int64_t kp = pad64(a.k);
+void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
+  const int64_t kp = pad64(a.k), most = round_tokens(a.tokens, a.k);
   char* p = (char*)workspace;
   float* qs = (float*)p;
-  p += pad256(a.tokens * 4);
+  p += pad256(most * 4);
   int8_t* q = (int8_t*)p;
-  p += pad256(a.tokens * kp);
+  p += pad256(most * kp);
   int8_t* wp = (int8_t*)p;
   Int8Gemm g{};
   g.q = q; g.qs = qs; g.kp = kp;
-  g.w = a.w; g.w_row = a.w_row; g.kw = a.k;
+  g.w = a.w; g.w_row = a.w_row; g.w_panel = 64;
+  g.w_bytes = (int64_t)(a.n - 1) * a.w_row + a.k;
   g.ws = a.w_scale; g.bias = a.bias;
   g.out = a.out; g.out_row = a.out_row;
   g.tokens = a.tokens; g.n = a.n;
@@ -442,25 +483,38 @@ void launch_int8_t(const Int8Args& a, void* workspace, hipStream_t s) {
     }
     return;
   }
-  launch_quant_rows<T>(a, kp, q, qs, s);
-  // rows that 16-byte loads at 32-bit offsets cannot address are laid out again
-  // (k % 4: the loads' bounds check drops a dword that ends past the last row)
-  if (a.k % 4 || a.w_row % 16 || (uintptr_t)a.w % 16 || a.w_row > (1 << 20)) {
-    hipLaunchKernelGGL(repack_kernel, dim3(a.n), dim3(256), 0, s, a.w, a.w_row, a.k, kp, wp);
+  // The weights as panels where many token tiles read them, and where 16-byte
+  // loads at 32-bit offsets cannot address their rows (k % 4: the loads' bounds
+  // check drops a dword that ends past the last row).
+  const bool four = a.k % 4 == 0 && a.w_row % 4 == 0 && (uintptr_t)a.w % 4 == 0;
+  if (a.tokens >= kPanelTokens || !four || a.w_row % 16 || (uintptr_t)a.w % 16 || g.w_bytes > 0x7fffffff) {
+    const dim3 grid((a.n + 15) / 16, (unsigned)(kp / 64));
+    if (four) hipLaunchKernelGGL((panels_kernel<true>), grid, dim3(256), 0, s, a.w, a.w_row, a.n, a.k, wp);
+    else hipLaunchKernelGGL((panels_kernel<false>), grid, dim3(256), 0, s, a.w, a.w_row, a.n, a.k, wp);
     g.w = wp;
-    g.w_row = g.kw = kp;
+    g.w_row = 64;
+    g.w_panel = (int64_t)a.n * 64;
+    g.w_bytes = a.n * kp;
   }
-  const int64_t t256 = (a.tokens + 255) / 256 * ((a.n + 127) / 128), t128 = (a.tokens + 127) / 128 * ((a.n + 127) / 128);
-  if (t256 >= 512) launch_tiles<T, 4, 2, 3>(g, s);
-  else if (t128 >= 256) launch_tiles<T, 2, 2, 4>(g, s);
-  else launch_tiles<T, 1, 1, 4>(g, s);
+  for (int64_t t0 = 0; t0 < a.tokens; t0 += most) {
+    Int8Args r = a;
+    r.tokens = g.tokens = std::min(most, a.tokens - t0);
+    r.x = (const char*)a.x + t0 * a.x_row * (T == kOpF32 ? 4 : 2);
+    g.out = (char*)a.out + t0 * a.out_row * (T == kOpF32 ? 4 : 2);
+    launch_quant_rows<T>(r, kp, q, qs, s);
+    const int64_t t256 = (r.tokens + 255) / 256 * ((a.n + 127) / 128), t128 = (r.tokens + 127) / 128 * ((a.n + 127) / 128);
+    if (t256 >= 512) launch_tiles<T, 4, 2, 3>(g, s);
+    else if (t128 >= 256) launch_tiles<T, 2, 2, 4>(g, s);
+    else launch_tiles<T, 1, 1, 4>(g, s);
+  }
 }
 
 }  // namespace
 
 int64_t int8_workspace(int64_t tokens, int64_t k, int64_t n) {
   if (tokens <= 0 || k <= 0 || n <= 0) return 0;
-  return pad256(tokens * 4) + pad256(tokens * pad64(k)) + pad256(n * pad64(k));
+  const int64_t most = round_tokens(tokens, k);
+  return pad256(most * 4) + pad256(most * pad64(k)) + pad256(n * pad64(k));
 }
 
 void launch_int8(const Int8Args& a, void* workspace, hipStream_t s) {

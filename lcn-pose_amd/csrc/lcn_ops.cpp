@@ -226,6 +226,7 @@ static int int8_sizes(const char* who, int64_t tokens, int64_t k, int64_t n) {
   if (k > kInt8MaxK) return fail(who, "k " + std::to_string(k) + " > 131072 (a 32-bit sum could overflow)");
   if (n > ((int64_t)1 << 24) || tokens > ((int64_t)1 << 30)) return fail(who, "too many channels (2^24) or tokens (2^30)");
   if (((tokens + 127) / 128) * ((n + 127) / 128) > ((int64_t)1 << 23)) return fail(who, "tokens x channels too large (2^37)");
+  if (n * (k + 63) > ((int64_t)1 << 31) - 64) return fail(who, "weight too large (2^31 bytes)");
   return LCN_OK;
 }
 

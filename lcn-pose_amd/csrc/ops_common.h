@@ -18,15 +18,10 @@ __device__ __forceinline__ float op_load(const void* p, int64_t e) {
   else if constexpr (T == kOpBF16) return __uint_as_float((unsigned)((const unsigned short*)p)[e] << 16);
   else return (float)((const _Float16*)p)[e];
 }
-__device__ __forceinline__ unsigned short bf16_bits(float v) {
-  unsigned u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40u);  // NaN stays a NaN
-  return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
 template <int T>
 __device__ __forceinline__ void op_store(void* p, int64_t e, float v) {
   if constexpr (T == kOpF32) ((float*)p)[e] = v;
-  else if constexpr (T == kOpBF16) ((unsigned short*)p)[e] = bf16_bits(v);
+  else if constexpr (T == kOpBF16) ((__bf16*)p)[e] = (__bf16)v;
   else ((_Float16*)p)[e] = (_Float16)v;
 }
 
