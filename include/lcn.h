@@ -116,6 +116,29 @@ int lcn_synchronize(void* handle);
  * Dropout; TF's own random stream cannot be reproduced. */
 int lcn_set_dropout(void* handle, float rate, uint64_t seed);
 
+/* The optimiser of the hidden weights (w2_l, w3_l) from the next step on; every
+ * other variable stays with Adam.  LCN_OPT_MUON: lcn_muon_update on the 2 L
+ * matrices of 17F x 17F with the gradients of the clipped, masked weights, the
+ * decayed learning rate, scale 0.2 sqrt(17F) and Muon's coefficients; the
+ * momentum takes the place of Adam's m for these weights
+ * (lcn_get/set_optimizer_state; their v is not used).  momentum in [0, 1), steps
+ * in [1, 64].  LCN_OPT_ADAM (the state after lcn_create) ignores the other
+ * arguments.  Replicas of several ranks stay equal: the update follows the
+ * all-reduced gradients.  No counterpart in the reference (Adam only,
+ * models_att.py:404-409). */
+enum { LCN_OPT_ADAM = 0, LCN_OPT_MUON = 1 };
+int lcn_set_optimizer(void* handle, int32_t kind, float momentum, int32_t nesterov, float weight_decay,
+                      int32_t steps);
+/* How lcn_forward, lcn_forward_loss and lcn_predict_dataset multiply the hidden
+ * layers: LCN_PRECISION_F32 (the state after lcn_create), or LCN_PRECISION_INT8:
+ * 8-bit integers with one scale a pose and one an output channel (the rounding
+ * rules of lcn_int8_linear), from the current weights at every call; the
+ * integers' buffers are allocated at the first such call (17F bytes a pose).
+ * Training steps, BatchNorm, the lift and the output layer stay in float32.  No
+ * counterpart in the reference (float32, models_att.py:79-132). */
+enum { LCN_PRECISION_F32 = 0, LCN_PRECISION_INT8 = 1 };
+int lcn_set_precision(void* handle, int32_t precision);
+
 /* --- device-resident data (on-device datasets; no host copies per step) */
 int lcn_device_buffer(void* handle, int32_t slot, int64_t bytes, void** dptr);
 int lcn_memcpy_h2d(void* handle, void* dst, const void* src, int64_t bytes);

@@ -270,7 +270,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ theta, fl
                                                    const float* __restrict__ M,
                                                    const float* __restrict__ lcoef, float reg,
                                                    const float* __restrict__ lr_t_dev, float beta1,
-                                                   float beta2, float eps, int update) {
+                                                   float beta2, float eps, int update,
+                                                   float* __restrict__ gmuon) {
   const int64_t b = blockIdx.x;
   int lo = 0, hi = nseg - 1;
   while (lo < hi) {
@@ -296,6 +297,10 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ theta, fl
     }
     if (sg.reg) g += reg * th;
     if (gout) gout[o] = g;
+    if (sg.muon) {  // the orthogonalised update follows (launch_ns)
+      gmuon[o] = g;
+      continue;
+    }
     if (update) {
       float mm = m[o], vv = v[o];
       mm += (g - mm) * omb1;
@@ -310,10 +315,10 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ theta, fl
 void launch_adam(float* theta, float* m, float* v, const float* rg, float* gout,
                  const AdamSeg* segs, const int64_t* seg_block_start, int nseg,
                  int64_t total_blocks, const float* M, const float* lcoef, float reg,
-                 const float* lr_t_dev, float beta1, float beta2, float eps, int update, hipStream_t s) {
+                 const float* lr_t_dev, float beta1, float beta2, float eps, int update, float* gmuon, hipStream_t s) {
   hipLaunchKernelGGL(adam_kernel, dim3((unsigned)total_blocks), dim3(256), 0, s, theta, m, v, rg,
                      gout, segs, seg_block_start, nseg, M, lcoef, reg, lr_t_dev, beta1, beta2, eps,
-                     update);
+                     update, gmuon);
 }
 
 }  // namespace lcn

@@ -23,6 +23,7 @@
 
 #include "../../include/lcn.h"
 #include "lcn_internal.h"
+#include "lcn_ops.h"
 
 using namespace lcn;
 
@@ -134,6 +135,20 @@ struct Handle {
   int64_t* seg_start = nullptr;
   int nseg = 0;
   int64_t adam_blocks = 0;
+
+  // optimiser of the hidden weights (lcn_set_optimizer): Adam, or Muon, whose
+  // momentum takes the place of Adam's m there
+  int optimizer = LCN_OPT_ADAM;
+  float mu_beta = 0.95f, mu_decay = 0.f;
+  int mu_nesterov = 1, mu_steps = 5;
+  AdamSeg* segs_muon = nullptr;   // the segments with the hidden weights marked
+  float* lr_muon = nullptr;       // the running step's learning rate (no bias correction)
+  void* mu_ws = nullptr;
+
+  // precision of the hidden layers' products in predictions (lcn_set_precision)
+  int precision = LCN_PRECISION_F32;
+  int8_t *q8 = nullptr, *w8 = nullptr;   // [nslab][rows][64] activations, [2L][nblk][4096] weights
+  float *qs8 = nullptr, *ws8 = nullptr;  // scales: a pose, [2L][H] channels
 
   // last batch
   int64_t lastB = 0;
@@ -1000,6 +1015,33 @@ int gemm_dw(Handle* h, const Operand& A, const Operand& D, const int2* blk, int 
   return LCN_OK;
 }
 
+// hidden layer k in 8-bit integers: X (raw, or through BN layer X.layer) -> Z[k]
+int int8_hidden(Handle* h, int k, const Operand& X, int epi_mode, int B) {
+  const bool bn = X.mode == PRO_BNACT;
+  hipEvent_t ev[2];
+  tstart(h, LCN_K_GEMM_FWD, ev);
+  launch_quant_tiles(X.p, X.S, B, bn ? h->bn[X.layer].scale : nullptr, bn ? h->bn[X.layer].shift : nullptr, h->F,
+                     h->alpha, h->q8, h->qs8, h->stream);
+  GemmArgs a{};
+  a.ptr = h->fwd_ptr;
+  a.idx = h->fwd_idx;
+  a.n_blocks = h->nblk;
+  a.bias = h->theta + h->b_off[k];
+  a.alpha = h->alpha;
+  a.Y = h->Z[k];
+  a.S_out = h->nslab;
+  a.epi_mode = epi_mode;
+  a.stat = epi_mode != EPI_NONE ? h->stat_part : nullptr;
+  a.epi_F = h->F;
+  a.B = B;
+  a.n_out_slabs = h->nslab;
+  a.n_rt = (int)cdiv(B, kRT);
+  h->stat_rows = kGemmRows;
+  launch_int8_slabs(a, h->q8, h->qs8, h->w8 + (int64_t)(k - 1) * h->nblk * 4096, h->ws8 + (int64_t)(k - 1) * h->H, h->stream);
+  tstop(h, LCN_K_GEMM_FWD, ev, 2.0 * 4096.0 * h->nblk * B);
+  return LCN_OK;
+}
+
 // BN + LeakyReLU backward of BN layer k from the EPI_BNBACK partials (sum du,
 // sum du*zhat) the GEMM producing its incoming gradient wrote: the dz
 // coefficients c123 (consumed by the PRO_BNBACK prologues), the BN parameter
@@ -1065,6 +1107,9 @@ int forward(Handle* h, int B, bool with_labels, bool train) {
   // the ranks' batch rows: with BatchNorm they ride on BN layer 0's all-reduce (bn_stats)
   if (!h->batch_norm) CHECK(exchange_rows(h, B));
   CHECK(prep_weights(h));
+  const bool int8 = !train && h->precision == LCN_PRECISION_INT8;
+  if (int8)  // from this call's fp32 blocks
+    launch_quant_blocks(h->wprep_items, 2 * h->L, S, h->fwd_ptr, h->fwd_idx, h->nblk, h->w8, h->ws8, s);
   const int epi = h->batch_norm ? EPI_BNFWD : EPI_NONE;
   // lift z0 = x . W1e + b1 (models_att.py:714-729): x padded to one 64-wide slab
   // the thin layers are HBM-bound: their timers accumulate algorithmic bytes
@@ -1078,7 +1123,8 @@ int forward(Handle* h, int B, bool with_labels, bool train) {
   // two_linear blocks (models_att.py:630-705)
   for (int l = 0; l < h->L; ++l) {
     const int k1 = 2 * l + 1, k2 = 2 * l + 2;
-    CHECK(gemm_hidden(h, k1, LCN_K_GEMM_FWD, raw(h->Hb[l], S), h->Z[k1], nullptr, epi, -1, B));
+    if (int8) CHECK(int8_hidden(h, k1, raw(h->Hb[l], S), epi, B));
+    else CHECK(gemm_hidden(h, k1, LCN_K_GEMM_FWD, raw(h->Hb[l], S), h->Z[k1], nullptr, epi, -1, B));
     CHECK(bn_stats(h, k1, B));
     // g = dropout(leaky(BN(z1))): fused into the next GEMM's operand load, or
     // materialised when dropout is on (the mask is per element, not per slab)
@@ -1088,7 +1134,8 @@ int forward(Handle* h, int B, bool with_labels, bool train) {
                     drop_of(h, k1, B), s);
       g = raw(h->Gb[l], S);
     }
-    CHECK(gemm_hidden(h, k2, LCN_K_GEMM_FWD, g, h->Z[k2], nullptr, epi, -1, B));
+    if (int8) CHECK(int8_hidden(h, k2, g, epi, B));
+    else CHECK(gemm_hidden(h, k2, LCN_K_GEMM_FWD, g, h->Z[k2], nullptr, epi, -1, B));
     CHECK(bn_stats(h, k2, B));
     bn_act_timed(h, h->Z[k2], h->residual ? h->Hb[l] : nullptr, h->Hb[l + 1], k2, B);
   }
@@ -1165,9 +1212,32 @@ int finish_device(Handle* h, bool update, bool keep_grads) {
   launch_wdot(h->rg, h->theta, h->w_offs, h->w_kin, h->w_nout, h->nl, h->blocksum, s);
   launch_maskgrad(h->blocksum, h->nl, h->Md, h->Sd, h->Cd, h->learnable, h->denom, h->norm2,
                   h->max_norm, h->learnable ? h->rg + h->mask_off : nullptr, h->lcoef, s);
-  launch_adam(h->theta, h->m, h->v, h->rg, keep_grads ? h->gout : nullptr, h->segs, h->seg_start,
+  const bool muon = h->optimizer == LCN_OPT_MUON;
+  launch_adam(h->theta, h->m, h->v, h->rg, keep_grads ? h->gout : nullptr, muon ? h->segs_muon : h->segs, h->seg_start,
               h->nseg, h->adam_blocks, h->Md, h->lcoef, h->reg, h->lr_dev, h->b1, h->b2, h->adam_eps,
-              update ? 1 : 0, s);
+              update ? 1 : 0, h->gout, s);
+  if (muon && update) {
+    // the hidden weights, equally spaced in the flat vector, as one batch of H x H matrices
+    const int64_t off = h->wl[1].w_off, stride = h->wl[2].w_off - off;
+    NsArgs a{};
+    a.batch = 2 * h->L;
+    a.rows = a.cols = h->H;
+    a.steps = h->mu_steps;
+    a.a = 3.4445f;
+    a.b = -4.775f;
+    a.c = 2.0315f;
+    a.eps = 1e-7f;
+    a.dtype = a.out_dtype = kOpF32;
+    a.in = MatView{h->gout + off, stride, h->H};
+    a.out = MatView{h->theta + off, stride, h->H};
+    a.momentum = MatView{h->m + off, stride, h->H};
+    a.beta = h->mu_beta;
+    a.nesterov = h->mu_nesterov;
+    a.lr_dev = h->lr_muon;
+    a.scale = 0.2f * sqrtf((float)h->H);
+    a.decay = h->mu_decay;
+    launch_ns(a, h->mu_ws, s);
+  }
   return LCN_OK;
 }
 
@@ -1444,6 +1514,10 @@ static int run_train_step(Handle* h, int64_t B, int32_t flags, float* loss_out, 
   uint32_t lr_bits;
   std::memcpy(&lr_bits, &lr_t, 4);
   HIPC(hipMemsetD32Async((hipDeviceptr_t)h->lr_dev, (int)lr_bits, 1, h->stream));
+  if (h->optimizer == LCN_OPT_MUON) {  // the decayed rate itself
+    std::memcpy(&lr_bits, &lr, 4);
+    HIPC(hipMemsetD32Async((hipDeviceptr_t)h->lr_muon, (int)lr_bits, 1, h->stream));
+  }
   hipGraphExec_t exec = nullptr;
   if (h->use_graphs && !multi(h) && !h->timing && h->drop_rate == 0.f &&
       step_graph(h, B, update, keep, &exec) != LCN_OK) {
@@ -1460,6 +1534,7 @@ static int run_train_step(Handle* h, int64_t B, int32_t flags, float* loss_out, 
     CHECK(enqueue_step(h, B, update, keep));
   }
   if (keep) h->grads_valid = 1;
+  else if (h->optimizer == LCN_OPT_MUON) h->grads_valid = 0;  // the step used the kept gradients' buffer
   if (update) {
     h->b1p *= h->b1;
     h->b2p *= h->b2;
@@ -1948,5 +2023,62 @@ extern "C" int lcn_set_dropout(void* handle, float rate, uint64_t seed) {
   h->drop_scale = 1.f / (1.f - rate);  // TF: scale = 1 / (1 - rate) in float32
   h->drop_seed = (uint32_t)seed ^ (uint32_t)(seed >> 32);
   h->drop_calls = 0;
+  return LCN_OK;
+}
+
+// The optimiser of the hidden weights from the next step on.  Captured step
+// graphs hold the old one's launches, so they go.
+extern "C" int lcn_set_optimizer(void* handle, int32_t kind, float momentum, int32_t nesterov, float weight_decay,
+                                 int32_t steps) {
+  Handle* h = (Handle*)handle;
+  if (!h) return LCN_E_ARG;
+  if (kind != LCN_OPT_ADAM && kind != LCN_OPT_MUON) { h->err = "unknown optimiser " + std::to_string(kind); return LCN_E_ARG; }
+  HIPC(hipSetDevice(h->device));
+  HIPC(hipStreamSynchronize(h->stream));
+  if (kind == LCN_OPT_MUON) {
+    if (!(momentum >= 0.f && momentum < 1.f)) { h->err = "Muon momentum must be in [0, 1)"; return LCN_E_ARG; }
+    if (!(weight_decay >= 0.f) || std::isinf(weight_decay)) { h->err = "Muon weight decay must be finite and >= 0"; return LCN_E_ARG; }
+    if (steps < 1 || steps > 64) { h->err = "Muon steps outside [1, 64]"; return LCN_E_ARG; }
+    if (h->L < 1) { h->err = "Muon needs a hidden layer (num_layers >= 1)"; return LCN_E_ARG; }
+    for (int k = 1; k <= 2 * h->L; ++k)
+      if (h->wl[k].w_off != h->wl[1].w_off + (k - 1) * (h->wl[2].w_off - h->wl[1].w_off)) {
+        h->err = "internal: hidden weights are not equally spaced";
+        return LCN_E_STATE;
+      }
+    if (!h->segs_muon) {
+      std::vector<AdamSeg> segs(h->nseg);
+      HIPC(hipMemcpy(segs.data(), h->segs, segs.size() * sizeof(AdamSeg), hipMemcpyDeviceToHost));
+      for (AdamSeg& sg : segs) sg.muon = sg.kind == 1 && h->wl[sg.layer].kind == 1;
+      CHECK(dalloc(h, &h->lr_muon, 1));
+      CHECK(dalloc(h, (char**)&h->mu_ws, (size_t)ns_workspace(2 * h->L, h->H, h->H)));
+      CHECK(upload(h, &h->segs_muon, segs));
+    }
+    h->mu_beta = momentum;
+    h->mu_nesterov = nesterov != 0;
+    h->mu_decay = weight_decay;
+    h->mu_steps = steps;
+  }
+  h->optimizer = kind;
+  for (auto& g : h->graphs) hipGraphExecDestroy(g.exec);
+  h->graphs.clear();
+  return LCN_OK;
+}
+
+// Precision of the hidden layers' products in predictions.
+extern "C" int lcn_set_precision(void* handle, int32_t precision) {
+  Handle* h = (Handle*)handle;
+  if (!h) return LCN_E_ARG;
+  if (precision != LCN_PRECISION_F32 && precision != LCN_PRECISION_INT8) { h->err = "unknown precision " + std::to_string(precision); return LCN_E_ARG; }
+  HIPC(hipSetDevice(h->device));
+  HIPC(hipStreamSynchronize(h->stream));
+  if (precision == LCN_PRECISION_INT8 && !h->ws8) {
+    const int64_t rows = cdiv(h->Bmax, kRT) * kRT;
+    if ((int64_t)h->nblk * 4096 > INT32_MAX) { h->err = "too many weight blocks for the int8 product"; return LCN_E_ARG; }
+    if (!h->q8) CHECK(dalloc(h, &h->q8, (size_t)rows * h->H));
+    if (!h->qs8) CHECK(dalloc(h, &h->qs8, (size_t)rows));
+    if (!h->w8) CHECK(dalloc(h, &h->w8, (size_t)2 * h->L * h->nblk * 4096));
+    CHECK(dalloc(h, &h->ws8, (size_t)2 * h->L * h->H));
+  }
+  h->precision = precision;
   return LCN_OK;
 }

@@ -547,6 +547,17 @@ void launch_maskgrad(const double* blocksum, int nl, const float* M, const float
                      const float* Cmat, int learnable, const float* denom, const double* norm2,
                      int max_norm, float* dV, float* lcoef, hipStream_t s);
 
+// The hidden layers of a prediction in 8-bit integers (kernels_int8_net.hip).
+// Activations X (row tiles of S slabs; scale / shift given: BN apply + LeakyReLU
+// first) -> q [S][ceil(B/32)*32][64], one scale a pose qs
+void launch_quant_tiles(const float* X, int S, int B, const float* scale, const float* shift, int F, float alpha, int8_t* q,
+                        float* qs, hipStream_t s);
+// the fp32 blocks of the hidden layers -> w8 [layer][block][64 outputs][64 inputs], ws [layer][nslab*64]
+void launch_quant_blocks(const WPrepHidden* items, int n_layers, int nslab, const int* ptr, const int2* idx, int nblk, int8_t* w8,
+                         float* ws, hipStream_t s);
+// z = (q . w8) qs ws + bias into a.Y (row tiles) with a's epilogue (EPI_NONE / EPI_BNFWD, 128-row partials)
+void launch_int8_slabs(const GemmArgs& a, const int8_t* q, const float* qs, const int8_t* w8, const float* ws, hipStream_t s);
+
 // Segment of the flat parameter vector for the fused gradient-finish + Adam.
 struct AdamSeg {
   int64_t off, size;
@@ -554,10 +565,11 @@ struct AdamSeg {
   int layer;               // weight: index into lcoef
   int cols, fin, fout;     // weight geometry
   int reg;                 // add regularisation * theta
+  int muon;                // hidden weight under Muon: write the gradient only
 };
 void launch_adam(float* theta, float* m, float* v, const float* rg, float* gout,
                  const AdamSeg* segs, const int64_t* seg_block_start, int nseg,
                  int64_t total_blocks, const float* M, const float* lcoef, float reg,
-                 const float* lr_t_dev, float beta1, float beta2, float eps, int update, hipStream_t s);
+                 const float* lr_t_dev, float beta1, float beta2, float eps, int update, float* gmuon, hipStream_t s);
 
 }  // namespace lcn

@@ -13,6 +13,7 @@ variable names the reference graph gives its variables (``tf_name_map``):
   linear_model/two_linear_<i>/{w2_<i>,b2_<i>,w3_<i>,b3_<i>}      (:630-705)
   linear_model/two_linear_<i>/batch_normalization{1,2}<i>/...    (:664-697)
   <var>/Adam, <var>/Adam_1                     AdamOptimizer slots m, v
+  <var>/Momentum                               instead, for the hidden weights under Muon
   beta1_power, beta2_power, global_step        Adam / training state (:386-409)
   loss/{mse_loss/Mean,add}/ExponentialMovingAverage
                                                loss EMA(0.9) shadows (:368-379):
@@ -73,15 +74,23 @@ def _ema_names(regularized: bool) -> Tuple[str, str]:
     return "loss/mse_loss/Mean", ("loss/add_1" if regularized else "loss/add")
 
 
+def _momentum(net, name: str) -> bool:
+    """Whether the optimiser state of variable `name` is Muon's momentum."""
+    return getattr(net, "optimizer", "adam") == "muon" and re.fullmatch(r"w[23]_\d+", name) is not None
+
+
 def to_tensors(net, loss_ema=None, regularized=False) -> Dict[str, np.ndarray]:
     params = net.get_params()
     m, v, gs, b1p, b2p = net.get_optimizer_state()
     t: Dict[str, np.ndarray] = {}
-    for _, tf, off, shape in tf_name_map(net.param_layout()):
+    for name, tf, off, shape in tf_name_map(net.param_layout()):
         n = int(np.prod(shape))
         t[tf] = params[off:off + n].reshape(shape).copy()
-        t[tf + "/Adam"] = m[off:off + n].reshape(shape).copy()
-        t[tf + "/Adam_1"] = v[off:off + n].reshape(shape).copy()
+        if _momentum(net, name):
+            t[tf + "/Momentum"] = m[off:off + n].reshape(shape).copy()
+        else:
+            t[tf + "/Adam"] = m[off:off + n].reshape(shape).copy()
+            t[tf + "/Adam_1"] = v[off:off + n].reshape(shape).copy()
         if tf.endswith("/gamma"):
             scope = tf[:-len("/gamma")]
             t[scope + "/moving_mean"] = np.zeros(shape, np.float32)
@@ -155,7 +164,11 @@ def restore(net, prefix: str) -> Optional[Tuple[float, int]]:
             raise ValueError(f"{tf}: checkpoint shape {t[tf].shape} != model shape {shape}")
         k = int(np.prod(shape))
         params[off:off + k] = t[tf].ravel()
-        if tf + "/Adam" in t:
+        # a slot of the other optimiser is not this one's state: it starts at zero
+        if _momentum(net, ours):
+            if tf + "/Momentum" in t:
+                m[off:off + k] = t[tf + "/Momentum"].ravel()
+        elif tf + "/Adam" in t:
             m[off:off + k] = t[tf + "/Adam"].ravel()
             v[off:off + k] = t[tf + "/Adam_1"].ravel()
     net.set_params(params)

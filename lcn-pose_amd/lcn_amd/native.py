@@ -20,6 +20,8 @@ MASK_LOCALLY_CONNECTED, MASK_EXPONENTIAL = 0, 1
 IN_DEVICE, OUT_DEVICE, NO_UPDATE, KEEP_GRADS, ASYNC = 1, 2, 4, 8, 16
 K_GEMM_FWD, K_GEMM_DX, K_GEMM_DW, K_BN_ACT, K_LIFT, K_OUT, K_OUT_DW, K_COMM = 0, 1, 2, 3, 4, 5, 6, 7
 DTYPE_F32, DTYPE_F64, DTYPE_BF16, DTYPE_F16 = 0, 1, 2, 3
+OPTIMIZERS = {"adam": 0, "muon": 1}
+PRECISIONS = {"fp32": 0, "int8": 1}
 MAX_DATASETS, MAX_COPIES = 16, 8
 AUG_NONE, AUG_FLIP, AUG_ROTATE, AUG_TRANSLATE = 0, 1, 2, 3
 
@@ -90,6 +92,8 @@ SIGNATURES = {
     "lcn_comm_info": ([_vp, ctypes.POINTER(_i32), ctypes.POINTER(_i32), ctypes.POINTER(_i32)], _i32),
     "lcn_crc32c": ([ctypes.c_uint32, ctypes.c_char_p, _i64], ctypes.c_uint32),
     "lcn_set_dropout": ([_vp, ctypes.c_float, ctypes.c_uint64], _i32),
+    "lcn_set_optimizer": ([_vp, _i32, ctypes.c_float, _i32, ctypes.c_float, _i32], _i32),
+    "lcn_set_precision": ([_vp, _i32], _i32),
     "lcn_eval_mpjpe": ([_i32, _i64, _f64p, _f64p, _f64p, _f64p, _f64p, _i32, _f64p], _i32),
     "lcn_eval_mpjpe_static": ([_i32, _i64, _f64p, _f64p, _f64p, _f64p, _f64p, _i32, _f64p], _i32),
     "lcn_orthogonalize_workspace": ([_i64, _i64, _i64], _i64),
@@ -230,6 +234,7 @@ class Network:
             raise LcnNativeError(f"lcn_create failed ({rc}): {self.lib.lcn_last_error(None).decode()}")
         self.h = h
         self.n_params = int(self.lib.lcn_num_params(self.h))
+        self.optimizer, self.precision = "adam", "fp32"
 
     # -- lifetime
     def close(self):
@@ -288,6 +293,22 @@ class Network:
                                                      ctypes.byref(gs), ctypes.byref(b1p),
                                                      ctypes.byref(b2p)))
         return m, v, gs.value, b1p.value, b2p.value
+
+    def set_optimizer(self, kind: str, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
+        """The optimiser of the hidden weights from the next step on: "adam", or "muon"
+        (lcn_set_optimizer; every other variable stays with Adam)."""
+        if kind not in OPTIMIZERS:
+            raise ValueError(f"unknown optimizer {kind!r}, expected one of {sorted(OPTIMIZERS)}")
+        self._check(self.lib.lcn_set_optimizer(self.h, OPTIMIZERS[kind], float(momentum), int(bool(nesterov)),
+                                               float(weight_decay), int(steps)))
+        self.optimizer = kind
+
+    def set_precision(self, precision: str):
+        """How predictions multiply the hidden layers: "fp32" or "int8" (lcn_set_precision)."""
+        if precision not in PRECISIONS:
+            raise ValueError(f"unknown precision {precision!r}, expected one of {sorted(PRECISIONS)}")
+        self._check(self.lib.lcn_set_precision(self.h, PRECISIONS[precision]))
+        self.precision = precision
 
     # -- compute
     def forward(self, x, out: Optional[np.ndarray] = None) -> np.ndarray:

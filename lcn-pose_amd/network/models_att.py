@@ -325,8 +325,13 @@ class cgcnn(base_model):
                  in_joints=17, out_joints=17, in_F=2, num_layers=2, residual=True, batch_norm=True,
                  max_norm=True, num_epochs=200, learning_rate=0.001, decay_type="exp",
                  decay_params=None, regularization=0.0, dropout=0, batch_size=200,
-                 eval_frequency=200, dir_name="", checkpoints="final", is_training=True, knn=1):
+                 eval_frequency=200, dir_name="", checkpoints="final", is_training=True, knn=1,
+                 optimizer="adam", precision="fp32"):
         super().__init__()
+        # not in the reference: "muon" orthogonalises the hidden weights' updates
+        # (Network.set_optimizer), "int8" multiplies the hidden layers of
+        # predictions in 8-bit integers (Network.set_precision)
+        self.optimizer, self.precision = optimizer, precision
         self.F = F
         self.mask_type = mask_type
         self.init_type = init_type
@@ -361,6 +366,10 @@ class cgcnn(base_model):
                             learning_rate=self.learning_rate, decay_steps=dp["decay_steps"],
                             decay_rate=dp["decay_rate"], max_batch=self.batch_size,
                             device=local)
+        if self.optimizer != "adam":
+            self._net.set_optimizer(self.optimizer)
+        if self.precision != "fp32":
+            self._net.set_precision(self.precision)
         if world > 1:
             # one process per GPU: RCCL communicator over the node's ranks; a
             # training step is then data parallel over each rank's shard

@@ -42,6 +42,11 @@ FLAGS = [
     ("--validation_set", str, {"train": None}, dict(choices=SETS, required=True)),
     ("--test_set", str, None, dict(choices=SETS, required={"train": False, "inference": True})),
     ("--n_test", int, {"train": 1}, dict(help="runs of a random search")),
+    # not in the reference; absent from the parsed arguments unless given
+    ("--optimizer", str, {"train": argparse.SUPPRESS},
+     dict(choices=["adam", "muon"], help="of the hidden weights (default adam)")),
+    ("--precision", str, {"inference": argparse.SUPPRESS},
+     dict(choices=["fp32", "int8"], help="of the hidden layers' products (default fp32)")),
 ]
 
 

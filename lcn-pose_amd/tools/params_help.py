@@ -70,6 +70,9 @@ def update_parameters(args, params):
         value = getattr(args, attr)
         if value:
             params[key] = value
+    for key in ("optimizer", "precision"):  # present only when given on the command line
+        if hasattr(args, key):
+            params[key] = getattr(args, key)
     for key in ("learning_rate", "regularization"):
         if hasattr(args, key):
             params[key] = getattr(args, key)
