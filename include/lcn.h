@@ -268,7 +268,8 @@ int lcn_eval_mpjpe_static(int32_t device, int64_t n, const double* pred, const d
  * thread's current device is unchanged.  They allocate nothing, do not
  * synchronise and may be captured into a graph.  Scratch memory is the
  * caller's: `workspace`, 256-byte aligned, at least as many bytes as the
- * matching _workspace function returns (negative: LCN_E_*); a workspace
+ * matching _workspace function returns (negative: LCN_E_*; 0: none needed,
+ * NULL will do); a workspace
  * belongs to one call at a time in stream order, so calls on two streams (or
  * two graphs that may run at once) need two.  dtype: LCN_DTYPE_F32, _BF16 or
  * _F16.  Matrices have a contiguous last dimension; strides are in elements

@@ -341,7 +341,8 @@ template <int T, bool kFused, bool kAligned>
 __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ int red[4][256];
-  __shared__ float qs[kFewTokens];
+  __shared__ float qs[kFewTokens], tops[4][4];
+  __shared__ int bads[4][4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int kp = (int)g.kp, tokens = (int)g.tokens;
   const int n0 = blockIdx.x * 16;
@@ -368,14 +369,32 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
     if (w + 4 * i < nk) wv[i] = weights(w + 4 * i);
   const int pitch = kp + 16;  // rows start 16 bytes apart in the banks
   if constexpr (kFused) {
-    for (int t = w; t < tokens; t += 4) {
-      float top = 0.f, factor, s;
+    // four rows at a time, one a wave, or (fewer tokens than waves) one row after
+    // another by the whole workgroup; up to kRegs elements a thread stay in registers
+    constexpr int kRegs = 8;
+    const bool wide = tokens < 4;
+    const int step = wide ? 256 : 64, at = wide ? threadIdx.x : lane;
+    for (int t = wide ? 0 : w; t < tokens; t += wide ? 1 : 4) {
+      float top = 0.f, factor, s, keep[kRegs];
       bool bad = false;
-      for (int c = lane; c < k; c += 64) see(op_load<T>(x, t * x_row + c), top, bad);
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) keep[i] = at + i * step < k ? op_load<T>(x, t * x_row + at + i * step) : 0.f;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) see(keep[i], top, bad);
+      for (int c = at + kRegs * step; c < k; c += step) see(op_load<T>(x, t * x_row + c), top, bad);
       wave_top(top, bad);
+      if (wide) {
+        if (lane == 0) { tops[t][w] = top; bads[t][w] = bad; }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { top = fmaxf(top, tops[t][i]); bad |= bads[t][i] != 0; }
+      }
       row_scale(top, bad, factor, s);
-      if (lane == 0) qs[t] = s;
-      for (int c = lane; c < kp; c += 64)
+      if (at == 0) qs[t] = s;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i)
+        if (at + i * step < kp) lds[t * pitch + at + i * step] = bad ? (char)0 : (char)quant(keep[i], factor);
+      for (int c = at + kRegs * step; c < kp; c += step)
         lds[t * pitch + c] = c < k && !bad ? (char)quant(op_load<T>(x, t * x_row + c), factor) : (char)0;
     }
     __syncthreads();
@@ -448,6 +467,11 @@ void launch_tiles(Int8Gemm& g, hipStream_t s) {
   hipLaunchKernelGGL((int8_gemm_kernel<T, BI, BJ, R>), dim3((unsigned)(tt * g.tn)), dim3(256), 0, s, g);
 }
 
+// every workgroup quantises the tokens for itself while that is little work
+bool fused(int64_t tokens, int64_t k) {
+  return tokens <= kFewTokens && tokens * (pad64(k) + 16) <= kFewLds && tokens * k <= 16384;
+}
+
 // Tokens of one quantise + multiply round: their integers stay below 1 GiB, which
 // 32-bit offsets reach.
 int64_t round_tokens(int64_t tokens, int64_t k) { return std::min(tokens, std::max<int64_t>(256, ((int64_t)1 << 30) / pad64(k) / 256 * 256)); }
@@ -472,8 +496,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
     const bool al = a.k % 16 == 0 && a.w_row % 16 == 0 && (uintptr_t)a.w % 16 == 0;
     const int64_t lds = a.tokens * (kp + 16);
     const dim3 grid((a.n + 15) / 16);
-    // every workgroup quantises the tokens for itself while that is little work
-    if (lds <= kFewLds && a.tokens * a.k <= 16384) {
+    if (fused(a.tokens, a.k)) {
       if (al) hipLaunchKernelGGL((int8_few_kernel<T, true, true>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
       else hipLaunchKernelGGL((int8_few_kernel<T, true, false>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
     } else {
@@ -513,6 +536,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
 
 int64_t int8_workspace(int64_t tokens, int64_t k, int64_t n) {
   if (tokens <= 0 || k <= 0 || n <= 0) return 0;
+  if (fused(tokens, k)) return 0;
   const int64_t most = round_tokens(tokens, k);
   return pad256(most * 4) + pad256(most * pad64(k)) + pad256(n * pad64(k));
 }

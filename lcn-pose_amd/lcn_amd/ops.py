@@ -26,23 +26,20 @@ MUON_COEFFICIENTS = (3.4445, -4.775, 2.0315)
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
 
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = load_library()
+    return _lib
+
+
 def _check(rc: int):
     if rc != 0:
-        message = load_library().lcn_last_error(None).decode()
+        message = _library().lcn_last_error(None).decode()
         raise ValueError(message) if rc == -1 else LcnNativeError(f"liblcn error {rc}: {message}")
-
-
-def _size(n: int) -> int:
-    if n < 0:
-        _check(n)
-    return n
-
-
-def _dtype(t: torch.Tensor, name: str) -> int:
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"{name} has type {t.dtype}, expected float32, bfloat16 or float16") from None
 
 
 def _expect(cond: bool, message: str):
@@ -50,27 +47,48 @@ def _expect(cond: bool, message: str):
         raise ValueError(message)
 
 
+def _dtype(t: torch.Tensor, name: str) -> int:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} has type {t.dtype}, expected float32, bfloat16 or float16")
+    return dt
+
+
 def _tensor(t, name: str, device=None) -> torch.Tensor:
-    _expect(isinstance(t, torch.Tensor), f"{name} is not a tensor")
-    _expect(t.is_cuda, f"{name} is on {t.device}: these operators run on the GPU only")
-    _expect(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
-    _expect(not (t.requires_grad and torch.is_grad_enabled()),
-            f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad()")
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} is not a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}: these operators run on the GPU only")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad()")
     return t
 
 
 def _matrices(t: torch.Tensor, name: str):
     """(batch, rows, cols, batch stride, row stride) of a [rows, cols] or [batch, rows, cols] tensor."""
-    _expect(t.dim() in (2, 3), f"{name} has {t.dim()} dimensions, expected [rows, cols] or [batch, rows, cols]")
-    s = t.stride()
-    _expect(t.shape[-1] <= 1 or s[-1] == 1, f"{name}'s last dimension is not contiguous")
-    if t.dim() == 2:
-        return 1, t.shape[0], t.shape[1], 0, s[0]
-    return t.shape[0], t.shape[1], t.shape[2], s[0], s[1]
+    shape, s = t.shape, t.stride()
+    if len(shape) not in (2, 3):
+        raise ValueError(f"{name} has {len(shape)} dimensions, expected [rows, cols] or [batch, rows, cols]")
+    if shape[-1] > 1 and s[-1] != 1:
+        raise ValueError(f"{name}'s last dimension is not contiguous")
+    if len(shape) == 2:
+        return 1, shape[0], shape[1], 0, s[0]
+    return shape[0], shape[1], shape[2], s[0], s[1]
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# the handle of torch's current stream of a device, without building a Stream object
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _workspace(size_of, a: int, b: int, c: int, device) -> torch.Tensor:
+    """Scratch memory of a call from torch's allocator, which knows the stream."""
+    n = size_of(a, b, c)
+    if n < 0:
+        _check(n)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 _coefficients = {}
@@ -78,13 +96,13 @@ _coefficients = {}
 
 def _triple(c):
     """The three coefficients as a C array (kept: the same few triples come again and again)."""
-    key = tuple(c)
-    a = _coefficients.get(key)
+    a = _coefficients.get(c) if type(c) is tuple else None
     if a is None:
-        _expect(len(key) == 3, "coefficients are three numbers (a, b, c)")
-        a = (ctypes.c_float * 3)(*[float(v) for v in key])
+        c = tuple(float(v) for v in c)
+        _expect(len(c) == 3, "coefficients are three numbers (a, b, c)")
+        a = (ctypes.c_float * 3)(*c)
         if len(_coefficients) < 64:
-            _coefficients[key] = a
+            _coefficients[c] = a
     return a
 
 
@@ -107,9 +125,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
         _tensor(out, "out", g.device)
         _expect(out.shape == g.shape and out.dtype == g.dtype, "out differs from g in shape or type")
     _, _, _, ob, orow = _matrices(out, "out")
-    lib = load_library()
-    ws = torch.empty(_size(lib.lcn_orthogonalize_workspace(n, r, c)), dtype=torch.uint8, device=g.device)
-    _check(lib.lcn_orthogonalize(g.device.index, _stream(g.device), dt, n, r, c, g.data_ptr(), sb, sr, out.data_ptr(),
+    lib, device = _library(), g.device.index
+    ws = _workspace(lib.lcn_orthogonalize_workspace, n, r, c, g.device)
+    _check(lib.lcn_orthogonalize(device, _stream(device), dt, n, r, c, g.data_ptr(), sb, sr, out.data_ptr(),
                                  ob, orow, int(steps), _triple(coefficients), eps, ws.data_ptr(), ws.numel()))
     return out
 
@@ -144,9 +162,9 @@ def muon_update(param: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor,
         lr_value = float(lr)
     if scale is None:
         scale = 0.2 * math.sqrt(max(r, c))
-    lib = load_library()
-    ws = torch.empty(_size(lib.lcn_orthogonalize_workspace(n, r, c)), dtype=torch.uint8, device=param.device)
-    _check(lib.lcn_muon_update(param.device.index, _stream(param.device), dt, n, r, c, param.data_ptr(), pb, pr,
+    lib, device = _library(), param.device.index
+    ws = _workspace(lib.lcn_orthogonalize_workspace, n, r, c, param.device)
+    _check(lib.lcn_muon_update(device, _stream(device), dt, n, r, c, param.data_ptr(), pb, pr,
                                momentum.data_ptr(), mb, mr, grad.data_ptr(), gb, gr, lr_value, lr_ptr, scale, beta,
                                int(nesterov), weight_decay, int(steps), _triple(coefficients), eps, ws.data_ptr(),
                                ws.numel()))
@@ -162,7 +180,7 @@ def quantize_weight(w: torch.Tensor, *, channel_dim: int = 0):
     n, k = w.shape[channel_dim], w.shape[1 - channel_dim]
     q = torch.empty(n, k, dtype=torch.int8, device=w.device)
     scale = torch.empty(n, dtype=torch.float32, device=w.device)
-    _check(load_library().lcn_int8_quantize_weight(w.device.index, _stream(w.device), dt, n, k, w.data_ptr(),
+    _check(_library().lcn_int8_quantize_weight(w.device.index, _stream(w.device.index), dt, n, k, w.data_ptr(),
                                                    w.stride(channel_dim), w.stride(1 - channel_dim), q.data_ptr(),
                                                    scale.data_ptr()))
     return q, scale
@@ -183,33 +201,38 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias
     _tensor(weight, "weight", dev)
     _tensor(scale, "scale", dev)
     dt = _dtype(x, "x")
-    _expect(weight.dtype == torch.int8 and weight.dim() == 2, "weight is an int8 matrix [n, k]")
+    shape = x.shape
+    if weight.dtype != torch.int8 or weight.dim() != 2:
+        raise ValueError("weight is an int8 matrix [n, k]")
     n, k = weight.shape
-    _expect(x.dim() >= 1 and x.shape[-1] == k, f"x ends in {tuple(x.shape[-1:])}, the weight has k = {k}")
-    _expect(k <= 1 or (x.stride(-1) == 1 and weight.stride(1) == 1), "the last dimension of x and weight is not contiguous")
-    _expect(scale.dtype == torch.float32 and scale.shape == (n,) and (n <= 1 or scale.stride(0) == 1),
-            f"scale is a contiguous float32 [{n}]")
+    ws_row, ws_col = weight.stride()
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x ends in {tuple(shape[-1:])}, the weight has k = {k}")
+    if k > 1 and (x.stride(-1) != 1 or ws_col != 1):
+        raise ValueError("the last dimension of x and weight is not contiguous")
+    if scale.dtype != torch.float32 or scale.shape != (n,) or not scale.is_contiguous():
+        raise ValueError(f"scale is a contiguous float32 [{n}]")
     bias_ptr = None
     if bias is not None:
         _tensor(bias, "bias", dev)
-        _expect(bias.dtype == torch.float32 and bias.shape == (n,) and (n <= 1 or bias.stride(0) == 1),
-                f"bias is a contiguous float32 [{n}]")
+        if bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias is a contiguous float32 [{n}]")
         bias_ptr = bias.data_ptr()
-    x2 = x if x.dim() == 2 else _rows(x, "x")
-    shape = x.shape[:-1] + (n,)
+    x2 = x if len(shape) == 2 else _rows(x, "x")
+    tokens = x2.shape[0]
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out2 = torch.empty((tokens, n), dtype=x.dtype, device=dev)
+        out = out2 if len(shape) == 2 else out2.view(shape[:-1] + (n,))
     else:
         _tensor(out, "out", dev)
-        _expect(out.shape == shape and out.dtype == x.dtype, f"out is a {x.dtype} {tuple(shape)}")
+        _expect(out.shape == shape[:-1] + (n,) and out.dtype == x.dtype, f"out is a {x.dtype} {tuple(shape[:-1]) + (n,)}")
         _expect(n <= 1 or out.stride(-1) == 1, "out's last dimension is not contiguous")
-    out2 = out if out.dim() == 2 else _rows(out, "out")
-    tokens = x2.shape[0]
-    lib = load_library()
-    ws = torch.empty(_size(lib.lcn_int8_linear_workspace(tokens, k, n)), dtype=torch.uint8, device=dev)
-    _check(lib.lcn_int8_linear(dev.index, _stream(dev), dt, tokens, k, n, x2.data_ptr(), x2.stride(0),
-                               weight.data_ptr(), weight.stride(0), scale.data_ptr(), bias_ptr, out2.data_ptr(),
-                               out2.stride(0), ws.data_ptr(), ws.numel()))
+        out2 = out if out.dim() == 2 else _rows(out, "out")
+    lib, device = _library(), dev.index
+    ws = _workspace(lib.lcn_int8_linear_workspace, tokens, k, n, dev)
+    _check(lib.lcn_int8_linear(device, _stream(device), dt, tokens, k, n, x2.data_ptr(), x2.stride(0), weight.data_ptr(),
+                               ws_row, scale.data_ptr(), bias_ptr, out2.data_ptr(), out2.stride(0), ws.data_ptr(),
+                               ws.numel()))
     return out
 
 

@@ -77,7 +77,7 @@ def test_muon_update_refuses(lib, kw, word):
 
 
 def _int8(lib, **kw):
-    a = dict(dtype=F32, t=4, k=32, n=16, x=A, xr=32, w=B, wr=32, s=C, b=None, out=4 << 32, orow=16, ws=WS, wsb=BIG)
+    a = dict(dtype=F32, t=40, k=32, n=16, x=A, xr=32, w=B, wr=32, s=C, b=None, out=4 << 32, orow=16, ws=WS, wsb=BIG)
     a.update(kw)
     return lib.lcn_int8_linear(0, None, a["dtype"], a["t"], a["k"], a["n"], a["x"], a["xr"], a["w"], a["wr"], a["s"],
                                a["b"], a["out"], a["orow"], a["ws"], a["wsb"])
