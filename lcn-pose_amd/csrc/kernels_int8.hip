@@ -39,9 +39,11 @@ __device__ __forceinline__ int quant(float v, float factor) {
 
 // 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
 template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
-template <int T>
+// (kOnce: not kept in the caches, which then hold the integers for the product)
+template <int T, bool kOnce>
 __device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {
-  const v4u u = *(const v4u*)((const char*)p + e * (16 / kVec<T>));
+  const v4u* at = (const v4u*)((const char*)p + e * (16 / kVec<T>));
+  const v4u u = kOnce ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (T == kOpF32) v[i] = __uint_as_float(u[i]);
@@ -65,10 +67,13 @@ __device__ __forceinline__ void see(float v, float& top, bool& bad) {
 }
 
 // One wave a row: largest magnitude, then the integers, rows padded to kp with
-// zeros.  kAligned: rows of whole 16-byte pieces; up to kRegs pieces a lane stay
-// in registers between the two passes, the rest is read again (from L2).
-// Bound by the read of x: 65 536 x 1088 fp32 in .. us.
-template <int T, bool kAligned>
+// zeros.  kPieces > 0: rows of whole 16-byte pieces, of which a lane keeps up to
+// kPieces in registers between the two passes; what is past them is read again
+// (from L2).  kPieces = 0: any alignment, an element at a time.  Bound by memory:
+// 65 536 x 1088 fp32 in 60 us (5.9 TB/s).  x is read past the caches: with it in
+// them, the integers had to come from memory again (77 us here, and 140 instead
+// of 98 us in the product).
+template <int T, int kPieces>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict__ x, int64_t x_row, int64_t tokens, int k,
                                                          int64_t kp, int8_t* __restrict__ q, float* __restrict__ scale) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -79,13 +84,13 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
   const int64_t r = t * x_row;
   int8_t* out = q + t * 64;
   const int64_t panel = tokens * 64;
-  if constexpr (kAligned) {
-    constexpr int V = kVec<T>, kRegs = 6;
+  if constexpr (kPieces > 0) {
+    constexpr int V = kVec<T>, kRegs = kPieces;
     const int pieces = k / V;  // k is a multiple of V here
     float keep[kRegs][V];
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) {
-      if (lane + 64 * i < pieces) load_vec<T>(x, r + (int64_t)(lane + 64 * i) * V, keep[i]);
+      if (lane + 64 * i < pieces) load_vec<T, true>(x, r + (int64_t)(lane + 64 * i) * V, keep[i]);
       else
 #pragma unroll
         for (int e = 0; e < V; ++e) keep[i][e] = 0.f;
@@ -96,7 +101,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
       for (int e = 0; e < V; ++e) see(keep[i][e], top, bad);
     for (int c = lane + 64 * kRegs; c < pieces; c += 64) {
       float v[V];
-      load_vec<T>(x, r + (int64_t)c * V, v);
+      load_vec<T, false>(x, r + (int64_t)c * V, v);
 #pragma unroll
       for (int e = 0; e < V; ++e) see(v[e], top, bad);
     }
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
       if (lane + 64 * i < padded) put(lane + 64 * i, keep[i]);
     for (int c = lane + 64 * kRegs; c < padded; c += 64) {
       float v[V] = {};
-      if (c < pieces) load_vec<T>(x, r + (int64_t)c * V, v);
+      if (c < pieces) load_vec<T, false>(x, r + (int64_t)c * V, v);
       put(c, v);
     }
   } else {
@@ -456,8 +461,10 @@ void launch_quant_rows(const Int8Args& a, int64_t kp, int8_t* q, float* qs, hipS
   constexpr int V = kVec<T>;
   const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && (a.x_row % V == 0 || a.tokens == 1);
   const dim3 grid((unsigned)((a.tokens + 3) / 4));
-  if (al) hipLaunchKernelGGL((quant_rows_kernel<T, true>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
-  else hipLaunchKernelGGL((quant_rows_kernel<T, false>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  constexpr int kMany = T == kOpF32 ? 18 : 9;  // K up to 4608 in registers
+  if (al && a.k <= 64 * 5 * V) hipLaunchKernelGGL((quant_rows_kernel<T, 5>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  else if (al) hipLaunchKernelGGL((quant_rows_kernel<T, kMany>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  else hipLaunchKernelGGL((quant_rows_kernel<T, 0>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
 }
 
 template <int T, int BI, int BJ, int R>

@@ -43,7 +43,10 @@ __global__ __launch_bounds__(64 * kQuantWaves) void quant_tiles_kernel(const flo
   const float4* x = (const float4*)(X + (size_t)rt * S * 2048);
   auto load = [&](int si, float4 (&v)[8]) {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) v[g] = x[si * 512 + g * 64 + lane];
+    for (int g = 0; g < 8; ++g) {  // read past the caches: they hold the integers for the product
+      const v4f_t u = __builtin_nontemporal_load((const v4f_t*)(x + si * 512 + g * 64 + lane));
+      v[g] = make_float4(u.x, u.y, u.z, u.w);
+    }
     if constexpr (kBn) {
       const int ch = (si % spj) * kSlab + 4 * h;
 #pragma unroll

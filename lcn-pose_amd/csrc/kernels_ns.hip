@@ -3,6 +3,7 @@
 //
 //   X0 = G / max(|G|_F, eps);  steps times:  A = X X^T,  B = b A + c A A,
 //   X <- a X + B X                            (on G^T where rows > cols)
+// (a joins B's diagonal, so X <- B X: the product reads no X beside its operand)
 //
 // The quintic pushes every singular value of X towards 1 (Muon: K. Jordan,
 // 2024; Newton-Schulz iterations: Bjorck & Bowie, 1971).  Muon's update:
@@ -181,10 +182,10 @@ struct NsProd {
   int64_t stride;                     // bytes between the matrices' workspaces
   int ti, tj;                         // tiles of P and Q that are whole
   int whole, rest;                    // tiles of a matrix: whole ones, ones with a partial row block
-  const char* E; int64_t e_lo;        // kSquare: A (= Q); kUpdate / kFinal: Xc, in (row j, contraction i) form
+  const char* E; int64_t e_lo;        // kSquare: A (= Q), in (row j, contraction i) form
   char* Y; int64_t y_lo;              // result in (row j, contraction i) form
   char* Z; int64_t z_lo;              // result in (row i, contraction j) form
-  float f, e;                         // result = f * sum + e * E  (scales of the stored forms folded in)
+  float f, e;                         // result = f * sum (+ e * E, + a on the diagonal: kSquare), in the stored forms' scales
 };
 
 #define NS_LDS(SRC, VOFF, SOFF, DST) \
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       for (int e = 0; e < 16; ++e) v[e] = acc[x][y][e] * g.f;
       // (row j, contraction i): octet 4 rbi + q of row block rbj, row l31, halves 4h .. 4h + 3
       const int64_t at = (((int64_t)rbj * (g.Rp / 8) + rbi * 4) * 32 + l31) * 16 + h * 8;
-      if constexpr (MODE != kGram) {
+      if constexpr (MODE == kSquare) {
         const char* E = g.E + mat * g.stride + at;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -356,6 +357,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 #pragma unroll
           for (int s2 = 0; s2 < 4; ++s2) v[4 * q + s2] = fmaf((float)eh[s2] + (float)el[s2], g.e, v[4 * q + s2]);
         }
+        if (rbi == rbj)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] += 8 * (e >> 2) + 4 * h + (e & 3) == l31 ? a.a * kSb : 0.f;
       }
       if constexpr (MODE == kFinal) {
         const bool tall = a.rows > a.cols;
@@ -528,15 +532,6 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
       *(half4*)(y + lo_at + q * 512) = lv;
     }
   };
-  auto get = [&](const char* from, int lo_at, int bj, int bi, float (&v)[16]) {
-    const char* y = from + ((bj * (M / 8) + bi * 4) * 32 + l31) * 16 + h * 8;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const half4 hv = *(const half4*)(y + q * 512), lv = *(const half4*)(y + lo_at + q * 512);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * q + e] = (float)hv[e] + (float)lv[e];
-    }
-  };
   // this wave's blocks of X X^T of the chunk in LDS, added to g
   auto gram = [&](f32x16 (&g)[G::GB]) {
 #pragma unroll
@@ -549,7 +544,7 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
       }
     }
   };
-  // A (scaled sums g) into sa, then B = b A + c A A in its place
+  // A (scaled sums g) into sa, then B = a I + b A + c A A in its place
   auto square = [&](f32x16 (&g)[G::GB]) {
     float v[G::GB][16];
 #pragma unroll
@@ -569,7 +564,10 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
         f32x16 acc = {}, cr = {};
         lds_product<M>(sa, G::kA, t % MB, sa, G::kA, t / MB, lane, acc, cr);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[k][e] = fmaf(acc[e] + cr[e], a.c * kSb / (kSa * kSa), v[k][e] * (a.b * kSb / kSa));
+        for (int e = 0; e < 16; ++e) {
+          v[k][e] = fmaf(acc[e] + cr[e], a.c * kSb / (kSa * kSa), v[k][e] * (a.b * kSb / kSa));
+          if (t / MB == t % MB && 8 * (e >> 2) + 4 * h + (e & 3) == l31) v[k][e] += a.a * kSb;
+        }
       }
     }
     __syncthreads();
@@ -580,7 +578,7 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
     }
     __syncthreads();
   };
-  // X <- a X + B X for the chunk in LDS; the last step writes the result
+  // X <- B X for the chunk in LDS; the last step writes the result
   auto update = [&](int ch, bool last) {
     float v[G::XB][16];
     const float sy = last ? 1.f : kSx;
@@ -590,9 +588,8 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
       if (t < MB * WB) {
         f32x16 acc = {}, cr = {};
         lds_product<M>(sa, G::kA, bi, sc, G::kX, bj, lane, acc, cr);
-        get(sc, G::kX, bj, bi, v[k]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[k][e] = fmaf(acc[e] + cr[e], sy / (kSb * kSx), v[k][e] * (a.a * sy / kSx));
+        for (int e = 0; e < 16; ++e) v[k][e] = (acc[e] + cr[e]) * (sy / (kSb * kSx));
       }
     }
     if (last) {
@@ -828,7 +825,7 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.y_lo = g.z_lo = p.aplane;
     g.f = kSa / (kSx * kSx);
     launch_prod<kGram, kOpF32>(g, a, p, s);
-    // B = b A + c A A
+    // B = a I + b A + c A A
     g.P = g.Q = g.E = ws + p.a;
     g.p_lo = g.q_lo = g.e_lo = p.aplane;
     g.K = p.mp;
@@ -836,10 +833,10 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.f = a.c * kSb / (kSa * kSa);
     g.e = a.b * kSb / kSa;
     launch_prod<kSquare, kOpF32>(g, a, p, s);
-    // X <- a X + B X
+    // X <- B X
     g.P = ws + p.b;
-    g.Q = g.E = xc;
-    g.q_lo = g.e_lo = p.xplane;
+    g.Q = xc;
+    g.q_lo = p.xplane;
     g.Rq = p.np;
     g.Y = yc;
     g.Z = yr;
@@ -847,7 +844,6 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     const bool last = k + 1 == a.steps;
     const float sy = last ? 1.f : kSx;
     g.f = sy / (kSb * kSx);
-    g.e = a.a * sy / kSx;
     if (last) launch_prod<kFinal, T>(g, a, p, s);
     else launch_prod<kUpdate, kOpF32>(g, a, p, s);
   }
