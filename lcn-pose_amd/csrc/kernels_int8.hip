@@ -189,8 +189,10 @@ template <int T, int BI, int BJ, int R>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void int8_gemm_kernel(Int8Gemm g) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass emits no launch stub for this body)
   constexpr int kRows = 64 * (BI + BJ), kStage = kRows * 64, L = BI + BJ;  // L: loads of a wave per stage
-  static_assert(R == 3 || R == 4, "ring depth");
-  __shared__ __attribute__((aligned(16))) char l0[kStage], l1[kStage], l2[kStage], l3[R == 4 ? kStage : 16];
+  static_assert(R == 3 || R == 4 || R == 8, "buffers named below");
+  constexpr int kFourth = R >= 4 ? kStage : 16, kRest = R == 8 ? kStage : 16;
+  __shared__ __attribute__((aligned(16))) char l0[kStage], l1[kStage], l2[kStage], l3[kFourth], l4[kRest], l5[kRest], l6[kRest], l7[kRest];
+#define I8_BUF(I) ((I) % R == 0 ? l0 : (I) % R == 1 ? l1 : (I) % R == 2 ? l2 : (I) % R == 3 ? l3 : (I) % R == 4 ? l4 : (I) % R == 5 ? l5 : (I) % R == 6 ? l6 : l7)
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int64_t t0 = (int64_t)(id / g.tn) * (64 * BI);
   const int n0 = (id % g.tn) * (64 * BJ);
@@ -266,35 +268,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
   };
   int ks = 0;
   if (nk >= 2 * R) {
-    stage(0, l0);
-    stage(1, l1);
-    stage(2, l2);
-    if constexpr (R == 4) stage(3, l3);
+#pragma unroll
+    for (int i = 0; i < R; ++i) stage(i, I8_BUF(i));
     stage_barrier<(R - 1) * L>();
     fetch(l0, 0, f0);
     do {
-      step(ks, l0, l1, true, true);
-      step(ks + 1, l1, l2, true, true);
-      step(ks + 2, l2, R == 4 ? l3 : l0, true, true);
-      if constexpr (R == 4) step(ks + 3, l3, l0, true, true);
+#pragma unroll
+      for (int i = 0; i < R; ++i) step(ks + i, I8_BUF(i), I8_BUF(i + 1), true, true);
       ks += R;
     } while (ks + 2 * R <= nk);
   } else {
-    stage(0, l0);
-    if (nk > 1) stage(1, l1);
-    if (nk > 2) stage(2, l2);
-    if (R == 4 && nk > 3) stage(3, l3);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i < nk) stage(i, I8_BUF(i));
     stage_barrier<0>();
     fetch(l0, 0, f0);
   }
   for (; ks < nk; ks += R) {  // at most 2 R - 1 stages remain
     const int left = nk - ks;
-    step(ks, l0, l1, left > 1, left > R);
-    if (left > 1) step(ks + 1, l1, l2, left > 2, left > R + 1);
-    if (left > 2) step(ks + 2, l2, R == 4 ? l3 : l0, left > 3, left > R + 2);
-    if constexpr (R == 4)
-      if (left > 3) step(ks + 3, l3, l0, left > 4, false);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (left > i) step(ks + i, I8_BUF(i), I8_BUF(i + 1), left > i + 1, left > R + i);
   }
+#undef I8_BUF
   // The tile of the output as a buffer: its rows end with the tile, so stores of
   // rows past the tokens are dropped, and lanes past the channels point behind it.
   // Row offsets are scalar: a store costs no address arithmetic.
@@ -535,7 +531,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
     const int64_t t256 = (r.tokens + 255) / 256 * ((a.n + 127) / 128), t128 = (r.tokens + 127) / 128 * ((a.n + 127) / 128);
     if (t256 >= 512) launch_tiles<T, 4, 2, 3>(g, s);
     else if (t128 >= 256) launch_tiles<T, 2, 2, 4>(g, s);
-    else launch_tiles<T, 1, 1, 4>(g, s);
+    else launch_tiles<T, 1, 1, 8>(g, s);
   }
 }
 

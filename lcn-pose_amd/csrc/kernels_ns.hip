@@ -192,11 +192,11 @@ struct NsProd {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
 
 // One tile of D = P Q^T with sides of 64 NB, four waves of 32 NB x 32 NB blocks;
-// K in steps of 16 (NB 2) or 32 (NB 1) through a ring of four LDS buffers filled
-// by LDS-DMA (16 KB a stage: hi and lo of both operands), three to four stages
-// in flight: with one stage in flight a
+// K in steps of 16 (NB 2) or 32 (NB 1) through a ring of four LDS buffers filled by
+// LDS-DMA (16 KB a stage: hi and lo of both operands), three to four stages in
+// flight (eight buffers measured the same, two 20 us for 12 where CUs are idle): with one stage in flight a
 // lone workgroup of a CU spent three quarters of its time waiting for the next
-// (46 us for six 1088 x 1088 Gram matrices).  The buffers are four LDS objects, and
+// (46 us for six 1088 x 1088 Gram matrices).  The buffers are LDS objects of their own, and
 // a stage's object is known at compile time, so the compiler adds no waits of
 // its own for loads into the others.
 template <int MODE, int T, int NB>
@@ -204,6 +204,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
   constexpr int KK = 2 / NB, TB = 2 * NB;  // 16-wide pieces of K a stage, row blocks of a tile's side
   __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
+#define NS_BUF(I) ((I) % R == 0 ? l0 : (I) % R == 1 ? l1 : (I) % R == 2 ? l2 : l3)
   // The whole tiles of all matrices come first, then those with fewer row blocks
   // of either operand.
   const int nwhole = g.whole * (int)a.batch;
@@ -302,37 +303,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     }
     multiply(cur);
   };
-  Frag f0, f1;
+  Frag f[2];
   int ks = 0;
   if (nk >= 2 * R) {  // (a block of its own: the compiler then knows how many loads are outstanding in the loop)
-    stage(0, l0);
-    stage(1, l1);
-    stage(2, l2);
-    stage(3, l3);
+#pragma unroll
+    for (int i = 0; i < R; ++i) stage(i, NS_BUF(i));
     stage_barrier<(R - 1) * L>();
-    fetch(l0, f0);
+    fetch(l0, f[0]);
     do {  // every step has a stage left to load
-      step(ks, l0, l1, f0, f1, true, true);
-      step(ks + 1, l1, l2, f1, f0, true, true);
-      step(ks + 2, l2, l3, f0, f1, true, true);
-      step(ks + 3, l3, l0, f1, f0, true, true);
+#pragma unroll
+      for (int i = 0; i < R; ++i) step(ks + i, NS_BUF(i), NS_BUF(i + 1), f[i & 1], f[(i + 1) & 1], true, true);
       ks += R;
     } while (ks + 2 * R <= nk);
   } else {
-    stage(0, l0);
-    if (nk > 1) stage(1, l1);
-    if (nk > 2) stage(2, l2);
-    if (nk > 3) stage(3, l3);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i < nk) stage(i, NS_BUF(i));
     stage_barrier<0>();
-    fetch(l0, f0);
+    fetch(l0, f[0]);
   }
-  for (; ks < nk; ks += R) {  // at most seven stages remain
+  for (; ks < nk; ks += R) {  // at most 2 R - 1 stages remain
     const int left = nk - ks;
-    step(ks, l0, l1, f0, f1, left > 1, left > 4);
-    if (left > 1) step(ks + 1, l1, l2, f1, f0, left > 2, left > 5);
-    if (left > 2) step(ks + 2, l2, l3, f0, f1, left > 3, left > 6);
-    if (left > 3) step(ks + 3, l3, l0, f1, f0, left > 4, false);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (left > i) step(ks + i, NS_BUF(i), NS_BUF(i + 1), f[i & 1], f[(i + 1) & 1], left > i + 1, left > R + i);
   }
+#undef NS_BUF
   if constexpr (NB == 1) acc[0][0] += cr;
   __syncthreads();
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
@@ -421,30 +417,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 
 // ---- matrices with a short side of at most 128 ---------------------------------------------
 // The short side's Gram matrix fits into LDS, so a workgroup does a whole step
-// for its own columns of X: A (from all workgroups' partial sums), B = b A + c A A
-// (every workgroup for itself), X <- a X + B X, and the next Gram matrix's
-// partial sum.  A step is one launch instead of three, and a matrix of few
-// columns is one launch in all.  X is held as chunks of W columns, each an LDS
-// image of Xc and Xr; a workgroup (slab) takes chunks slab, slab + S, ...
-// Bound by latency: launches, barriers and LDS round trips.
+// for its own columns of X: A (from all workgroups' partial sums), B = a I + b A +
+// c A A (every workgroup for itself), X <- B X, and the next Gram matrix's partial
+// sum.  A step is one launch instead of three, and a matrix of few columns is
+// one launch in all.  X is held as chunks of W columns, each an LDS image of Xc
+// and Xr; a workgroup (slab) takes chunks slab, slab + S, ...
+// Bound by latency (barriers, LDS round trips, cold code), so the work is spread
+// over NW waves in blocks of 16 x 16 (v_mfma_f32_16x16x32_f16: a lane supplies
+// row l % 16, k = 8 (l / 16) .. + 7 of either operand, which the planes' octets
+// hold, and receives four consecutive i of one j).
 enum { kSolo = 0, kFirst = 1, kMid = 2, kLast = 3 };
 
 struct ThinPlan {
   int m, n, chunks, slabs;
   int64_t grams, images, stride;  // per matrix: offsets of the partial sums (two sets) and the images; bytes
 };
-template <int MB, int WB>
+template <int MB, int WB, int NW>
 struct ThinGeo {
   static constexpr int M = 32 * MB, W = 32 * WB;
   static constexpr int kA = M * M * 2, kX = M * W * 2;     // bytes of a plane of A / B and of X
   static constexpr int kImage = 4 * kX;                    // Xc hi, Xc lo, Xr hi, Xr lo
   static constexpr int kLds = kImage + 2 * kA;
   static constexpr int kGram = M * M * 4;                  // bytes of a partial Gram matrix
-  static constexpr int GB = (MB * MB + 3) / 4, XB = (MB * WB + 3) / 4;  // 32 x 32 blocks a wave holds
+  static constexpr int kThreads = 64 * NW;
+  static constexpr int MT = M / 16, WT = W / 16;           // blocks along the sides
+  static constexpr int GB = MT * MT / NW, XB = MT * WT / NW;  // blocks a wave holds
+  static_assert(MT * MT % NW == 0 && MT * WT % NW == 0 && M * W % kThreads == 0 && kImage / 2 % (16 * kThreads) == 0, "");
 };
-template <int MB, int WB>
+template <int MB, int WB, int NW>
 ThinPlan make_thin(int64_t rows, int64_t cols) {
-  using G = ThinGeo<MB, WB>;
+  using G = ThinGeo<MB, WB, NW>;
   ThinPlan p;
   p.m = (int)std::min(rows, cols);
   p.n = (int)std::max(rows, cols);
@@ -456,151 +458,164 @@ ThinPlan make_thin(int64_t rows, int64_t cols) {
   return p;
 }
 
-// D += P Q^T for one 32 x 32 block: rows of block rp of plane pair P, rq of Q,
-// contraction length K; both LDS planes with their lo plane `lo` bytes behind
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// D += P Q^T for one 16 x 16 block: rows 16 rp .. of plane pair P, 16 rq .. of Q,
+// contraction length K; both in LDS with their lo plane behind by p_lo / q_lo
+// (three sums that do not wait for each other: hi hi, hi lo, lo hi)
 template <int K>
-__device__ __forceinline__ void lds_product(const char* P, int p_lo, int rp, const char* Q, int q_lo, int rq, int lane,
-                                            f32x16& acc, f32x16& cr) {
-  const char* p = P + rp * (K * 64) + lane * 16;
-  const char* q = Q + rq * (K * 64) + lane * 16;
+__device__ __forceinline__ void lds_product(const char* P, int p_lo, int rp, const char* Q, int q_lo, int rq, int lane, f32x4& acc) {
+  f32x4 cr = {}, cs = {};
+  const int at = (lane >> 4) * 512 + (lane & 15) * 16;
+  const char* p = P + (rp >> 1) * (K * 64) + (rp & 1) * 256 + at;
+  const char* q = Q + (rq >> 1) * (K * 64) + (rq & 1) * 256 + at;
 #pragma unroll
-  for (int kk = 0; kk < K / 16; ++kk) {
-    const half8 ph = *(const half8*)(p + kk * 1024), pl = *(const half8*)(p + p_lo + kk * 1024);
-    const half8 qh = *(const half8*)(q + kk * 1024), ql = *(const half8*)(q + q_lo + kk * 1024);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
-    cr = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, cr, 0, 0, 0);
-    cr = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, cr, 0, 0, 0);
+  for (int kk = 0; kk < K / 32; ++kk) {
+    const half8 ph = *(const half8*)(p + kk * 2048), pl = *(const half8*)(p + p_lo + kk * 2048);
+    const half8 qh = *(const half8*)(q + kk * 2048), ql = *(const half8*)(q + q_lo + kk * 2048);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    cr = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, cr, 0, 0, 0);
+    cs = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, cs, 0, 0, 0);
   }
+  acc += cr + cs;
 }
 
-template <int MB, int WB, int T, bool kMuon, int MODE>
-__global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int parts, const double* __restrict__ part,
-                                                      char* __restrict__ ws, int set) {
-  using G = ThinGeo<MB, WB>;
-  constexpr int M = G::M, W = G::W;
+template <int MB, int WB, int NW, int T, bool kMuon, int MODE>
+__global__ __launch_bounds__(64 * NW) void ns_thin_kernel(NsArgs a, ThinPlan p, int parts, const double* __restrict__ part,
+                                                          char* __restrict__ ws, int set) {
+  using G = ThinGeo<MB, WB, NW>;
+  constexpr int M = G::M, W = G::W, kThreads = G::kThreads;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char *sc = lds, *sr = lds + 2 * G::kX, *sa = lds + G::kImage;
-  __shared__ double red[4];
+  __shared__ double red[NW];
   const int64_t b = blockIdx.y;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, l31 = lane & 31;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, l4 = lane >> 4;
   const bool tall = a.rows > a.cols;
   char* mine = ws + b * p.stride;
 
-  // the source element of X's (i, j): the gradient, or muon's update direction
-  auto source = [&](int i, int j) {
-    const int64_t r = tall ? j : i, c = tall ? i : j;
-    float v = op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c);
-    if constexpr (kMuon) {
-      const float mo = ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c];
-      v = a.nesterov ? fmaf(a.beta, mo, v) : mo;
-    }
-    return v;
+  // This thread's elements of chunk `ch` of the source (the gradient, or muon's
+  // update direction), element e of the chunk at kThreads k + thread; zero outside
+  // the matrix.  All loads are in flight together.
+  constexpr int kMine = M * W / kThreads;
+  auto place = [&](int k, int& i, int& j) {
+    const int e = kThreads * k + threadIdx.x;
+    i = tall ? e % M : e / W;
+    j = tall ? e / M : e % W;
   };
-  // chunk `ch` of X0 into both LDS forms (zero outside the matrix)
-  auto load_source = [&](int ch, double norm2) {
+  auto load_source = [&](int ch, float (&v)[kMine]) {
+    float mo[kMuon ? kMine : 1];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      int i, j;
+      place(k, i, j);
+      const bool in = i < p.m && ch * W + j < p.n;
+      const int64_t r = tall ? ch * W + j : i, c = tall ? i : ch * W + j;
+      v[k] = in ? op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c) : 0.f;
+      if constexpr (kMuon) mo[k] = in ? ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c] : 0.f;
+    }
+    if constexpr (kMuon) {
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        if constexpr (MODE == kSolo) {  // (elsewhere the norm's launch updated the momentum)
+          int i, j;
+          place(k, i, j);
+          mo[k] = fmaf(a.beta, mo[k], v[k]);
+          if (i < p.m && j < p.n)
+            ((float*)a.momentum.p)[b * a.momentum.batch + (int64_t)(tall ? j : i) * a.momentum.row + (tall ? i : j)] = mo[k];
+        }
+        v[k] = a.nesterov ? fmaf(a.beta, mo[k], v[k]) : mo[k];
+      }
+    }
+  };
+  // byte offset of element (row, k) in a plane of contraction length K
+  auto half_at = [](int row, int k, int K) { return ((((row >> 5) * (K / 8) + (k >> 3)) * 32 + (row & 31)) * 8 + (k & 7)) * 2; };
+  // X0 from the source into both LDS forms
+  auto put_source = [&](const float (&v)[kMine], double norm2) {
     const double inv = (double)kSx / fmax(sqrt(norm2), (double)a.eps);
     const bool bad = !(norm2 < 1e300);
-#pragma unroll 8
-    for (int e = threadIdx.x; e < M * W; e += 256) {
-      const int i = tall ? e % M : e / W, j = tall ? e / M : e % W, gj = ch * W + j;
-      float v = i < p.m && gj < p.n ? source(i, gj) : 0.f;
-      v = bad ? __builtin_nanf("") : (float)((double)v * inv);
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      int i, j;
+      place(k, i, j);
       _Float16 hi, lo;
-      split(v, hi, lo);
-      char* c = sc + ((((j >> 5) * (M / 8) + (i >> 3)) * 32 + (j & 31)) * 8 + (i & 7)) * 2;
-      char* r = sr + ((((i >> 5) * (W / 8) + (j >> 3)) * 32 + (i & 31)) * 8 + (j & 7)) * 2;
+      split(bad ? __builtin_nanf("") : (float)((double)v[k] * inv), hi, lo);
+      char *c = sc + half_at(j, i, M), *r = sr + half_at(i, j, W);
       *(_Float16*)c = hi;
       *(_Float16*)(c + G::kX) = lo;
       *(_Float16*)r = hi;
       *(_Float16*)(r + G::kX) = lo;
     }
   };
-  // one block in (row j, contraction i) form into plane pair `to` of contraction length M
-  auto put = [&](char* to, int lo_at, int bj, int bi, const float (&v)[16]) {
-    char* y = to + ((bj * (M / 8) + bi * 4) * 32 + l31) * 16 + h * 8;
+  // one block (block row bi, block column bj) in (row j, contraction i) form into plane pair `to`
+  auto put = [&](char* to, int lo_at, int bj, int bi, f32x4 v) {
+    half4 hv, lv;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      half4 hv, lv;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        _Float16 hi, lo;
-        split(v[4 * q + e], hi, lo);
-        hv[e] = hi;
-        lv[e] = lo;
-      }
-      *(half4*)(y + q * 512) = hv;
-      *(half4*)(y + lo_at + q * 512) = lv;
+    for (int e = 0; e < 4; ++e) {
+      _Float16 hi, lo;
+      split(v[e], hi, lo);
+      hv[e] = hi;
+      lv[e] = lo;
     }
+    char* y = to + half_at(16 * bj + l15, 16 * bi + 4 * l4, M);
+    *(half4*)y = hv;
+    *(half4*)(y + lo_at) = lv;
   };
   // this wave's blocks of X X^T of the chunk in LDS, added to g
-  auto gram = [&](f32x16 (&g)[G::GB]) {
+  auto gram = [&](f32x4 (&g)[G::GB]) {
 #pragma unroll
     for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) {
-        f32x16 cr = {};
-        lds_product<W>(sr, G::kX, t % MB, sr, G::kX, t / MB, lane, g[k], cr);
-        g[k] += cr;
-      }
+      const int t = w + NW * k;
+      lds_product<W>(sr, G::kX, t % G::MT, sr, G::kX, t / G::MT, lane, g[k]);
     }
   };
   // A (scaled sums g) into sa, then B = a I + b A + c A A in its place
-  auto square = [&](f32x16 (&g)[G::GB]) {
-    float v[G::GB][16];
+  auto square = [&](f32x4 (&g)[G::GB]) {
 #pragma unroll
     for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) {
+      const int t = w + NW * k;
+      g[k] *= kSa / (kSx * kSx);
+      put(sa, G::kA, t / G::MT, t % G::MT, g[k]);
+    }
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[k][e] = g[k][e] * (kSa / (kSx * kSx));
-        put(sa, G::kA, t / MB, t % MB, v[k]);
+    for (int k = 0; k < G::GB; ++k) {
+      const int t = w + NW * k, bi = t % G::MT, bj = t / G::MT;
+      f32x4 acc = {};
+      lds_product<M>(sa, G::kA, bi, sa, G::kA, bj, lane, acc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[k][e] = fmaf(acc[e], a.c * kSb / (kSa * kSa), g[k][e] * (a.b * kSb / kSa));
+        if (bi == bj && 4 * l4 + e == l15) g[k][e] += a.a * kSb;
       }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) {
-        f32x16 acc = {}, cr = {};
-        lds_product<M>(sa, G::kA, t % MB, sa, G::kA, t / MB, lane, acc, cr);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          v[k][e] = fmaf(acc[e] + cr[e], a.c * kSb / (kSa * kSa), v[k][e] * (a.b * kSb / kSa));
-          if (t / MB == t % MB && 8 * (e >> 2) + 4 * h + (e & 3) == l31) v[k][e] += a.a * kSb;
-        }
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) put(sa, G::kA, t / MB, t % MB, v[k]);
+      const int t = w + NW * k;
+      put(sa, G::kA, t / G::MT, t % G::MT, g[k]);
     }
     __syncthreads();
   };
   // X <- B X for the chunk in LDS; the last step writes the result
   auto update = [&](int ch, bool last) {
-    float v[G::XB][16];
+    f32x4 v[G::XB];
     const float sy = last ? 1.f : kSx;
 #pragma unroll
     for (int k = 0; k < G::XB; ++k) {
-      const int t = w + 4 * k, bi = t % MB, bj = t / MB;
-      if (t < MB * WB) {
-        f32x16 acc = {}, cr = {};
-        lds_product<M>(sa, G::kA, bi, sc, G::kX, bj, lane, acc, cr);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[k][e] = (acc[e] + cr[e]) * (sy / (kSb * kSx));
-      }
+      const int t = w + NW * k;
+      v[k] = f32x4{};
+      lds_product<M>(sa, G::kA, t % G::MT, sc, G::kX, t / G::MT, lane, v[k]);
+      v[k] *= sy / (kSb * kSx);
     }
     if (last) {
       const float lr = kMuon ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
 #pragma unroll
       for (int k = 0; k < G::XB; ++k) {
-        const int t = w + 4 * k, bi = t % MB, j = ch * W + (t / MB) * 32 + l31;
-        if (t >= MB * WB || j >= p.n) continue;
+        const int t = w + NW * k, i0 = 16 * (t % G::MT) + 4 * l4, j = ch * W + 16 * (t / G::MT) + l15;
+        if (j >= p.n) continue;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = bi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+        for (int e = 0; e < 4; ++e) {
+          const int i = i0 + e;
           if (i >= p.m) continue;
           const int64_t o = b * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j);
           if constexpr (kMuon) {
@@ -616,16 +631,14 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < G::XB; ++k) {
-      const int t = w + 4 * k, bi = t % MB, bj = t / MB;
-      if (t >= MB * WB) continue;
+      const int t = w + NW * k, bi = t % G::MT, bj = t / G::MT;
       put(sc, G::kX, bj, bi, v[k]);
       // the (row i, contraction j) form, a half at a time
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i31 = 8 * (e >> 2) + 4 * h + (e & 3);
+      for (int e = 0; e < 4; ++e) {
         _Float16 hi, lo;
         split(v[k][e], hi, lo);
-        char* r = sr + (((bi * (W / 8) + bj * 4 + (l31 >> 3)) * 32 + i31) * 8 + (l31 & 7)) * 2;
+        char* r = sr + half_at(16 * bi + 4 * l4 + e, 16 * bj + l15, W);
         *(_Float16*)r = hi;
         *(_Float16*)(r + G::kX) = lo;
       }
@@ -633,30 +646,25 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
     __syncthreads();
   };
 
-  f32x16 g[G::GB] = {};
+  f32x4 g[G::GB] = {};
   if constexpr (MODE == kSolo) {
-    // the norm (and the momentum): every element once, then X0 from the same data
+    float v[kMine];
+    load_source(0, v);
     double s = 0.0;
-    for (int e = threadIdx.x; e < a.rows * a.cols; e += 256) {
-      const int r = e / a.cols, c = e - r * a.cols;
-      float v = op_load<T>(a.in.p, b * a.in.batch + (int64_t)r * a.in.row + c);
-      if constexpr (kMuon) {
-        float* mo = (float*)a.momentum.p + b * a.momentum.batch + (int64_t)r * a.momentum.row + c;
-        const float m1 = fmaf(a.beta, *mo, v);
-        *mo = m1;
-        v = a.nesterov ? fmaf(a.beta, m1, v) : m1;
-      }
-      s = fma((double)v, (double)v, s);
-    }
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) s = fma((double)v[k], (double)v[k], s);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (lane == 0) red[w] = s;
-    __syncthreads();  // (also orders the momentum written above before its reads below)
-    load_source(0, (red[0] + red[1]) + (red[2] + red[3]));
+    __syncthreads();
+    s = red[0];
+#pragma unroll
+    for (int q = 1; q < NW; ++q) s += red[q];
+    put_source(v, s);
     __syncthreads();
     for (int k = 0; k < a.steps; ++k) {
 #pragma unroll
-      for (int q = 0; q < G::GB; ++q) g[q] = {};
+      for (int q = 0; q < G::GB; ++q) g[q] = f32x4{};
       gram(g);
       square(g);
       update(0, k + 1 == a.steps);
@@ -672,35 +680,25 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
   auto load_image = [&](int ch) {
     const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc((void*)(mine + p.images + (int64_t)ch * G::kImage), 0, kBytes, 0x00020000);
 #pragma unroll
-    for (int e = 0; e < kBytes; e += 4096) NS_LDS(res, lane * 16, e + w * 1024, lds + e + w * 1024);
+    for (int e = 0; e < kBytes; e += 16 * kThreads) NS_LDS(res, lane * 16, e + w * 1024, lds + e + w * 1024);
   };
   if constexpr (MODE != kFirst) {
     load_image(slab);  // meanwhile: A from the slabs' partial sums, in slab order
 #pragma unroll
     for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) {
-        const float4* src = (const float4*)(gin + (t * 64 + lane) * 16);
-        constexpr int kAhead = 6, kPitch = G::kGram / 16;  // sums in flight
-        for (int q0 = 0; q0 < p.slabs; q0 += kAhead) {
-          float4 f[kAhead][4];
+      const f32x4* src = (const f32x4*)gin + (w + NW * k) * 64 + lane;
+      constexpr int kAhead = 12, kPitch = G::kGram / 16;  // sums in flight
+      for (int q0 = 0; q0 < p.slabs; q0 += kAhead) {
+        f32x4 f[kAhead];
 #pragma unroll
-          for (int q = 0; q < kAhead; ++q)
+        for (int q = 0; q < kAhead; ++q) f[q] = q0 + q < p.slabs ? src[(int64_t)(q0 + q) * kPitch] : f32x4{};
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              f[q][e] = q0 + q < p.slabs ? src[(int64_t)(q0 + q) * kPitch + e] : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int q = 0; q < kAhead; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              g[k][4 * e] += f[q][e].x; g[k][4 * e + 1] += f[q][e].y; g[k][4 * e + 2] += f[q][e].z; g[k][4 * e + 3] += f[q][e].w;
-            }
-        }
+        for (int q = 0; q < kAhead; ++q) g[k] += f[q];
       }
     }
     square(g);
 #pragma unroll
-    for (int q = 0; q < G::GB; ++q) g[q] = {};
+    for (int q = 0; q < G::GB; ++q) g[q] = f32x4{};
   }
   const double norm2 = MODE == kFirst ? norm2_of(part + b * kNormParts, parts) : 0.0;
   for (int ch = slab; ch < p.chunks; ch += p.slabs) {
@@ -709,24 +707,22 @@ __global__ __launch_bounds__(256) void ns_thin_kernel(NsArgs a, ThinPlan p, int 
       __syncthreads();  // the chunk before is done with
       if constexpr (MODE != kFirst) load_image(ch);
     }
-    if constexpr (MODE == kFirst) load_source(ch, norm2);
+    if constexpr (MODE == kFirst) {
+      float v[kMine];
+      load_source(ch, v);
+      put_source(v, norm2);
+    }
     __syncthreads();
     if constexpr (MODE != kFirst) update(ch, MODE == kLast);
     if constexpr (MODE != kLast) {
       gram(g);
-      for (int e = threadIdx.x; e < G::kImage / 16; e += 256) ((v4u*)image)[e] = ((const v4u*)lds)[e];
+#pragma unroll
+      for (int e = threadIdx.x; e < G::kImage / 16; e += kThreads) ((v4u*)image)[e] = ((const v4u*)lds)[e];
     }
   }
   if constexpr (MODE != kLast) {
 #pragma unroll
-    for (int k = 0; k < G::GB; ++k) {
-      const int t = w + 4 * k;
-      if (t < MB * MB) {
-        float4* dst = (float4*)(gout + (t * 64 + lane) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dst[e] = make_float4(g[k][4 * e], g[k][4 * e + 1], g[k][4 * e + 2], g[k][4 * e + 3]);
-      }
-    }
+    for (int k = 0; k < G::GB; ++k) ((f32x4*)gout)[(w + NW * k) * 64 + lane] = g[k];
   }
 }
 
@@ -739,30 +735,33 @@ int norm_parts(const NsArgs& a) {
   return std::max(1, std::min({kNormParts, (a.rows + 3) / 4, (int)std::max<int64_t>(1, 1024 / a.batch)}));
 }
 
-template <int MB, int WB, int T, bool kMuon>
+template <int MB, int WB, int NW, int T, bool kMuon>
 void launch_thin(const NsArgs& a, void* workspace, hipStream_t s) {
-  using G = ThinGeo<MB, WB>;
-  const ThinPlan p = make_thin<MB, WB>(a.rows, a.cols);
+  using G = ThinGeo<MB, WB, NW>;
+  const ThinPlan p = make_thin<MB, WB, NW>(a.rows, a.cols);
   double* part = (double*)workspace;
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
   if (p.chunks == 1) {
-    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kSolo>), dim3(1, (unsigned)a.batch), dim3(256), G::kLds, s, a, p, 0, part, ws, 0);
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kSolo>), dim3(1, (unsigned)a.batch), dim3(G::kThreads), G::kLds, s, a, p, 0, part, ws, 0);
     return;
   }
   const dim3 grid(p.slabs, (unsigned)a.batch);
   const int parts = norm_parts(a);
   launch_norm<T, kMuon>(a, parts, part, s);
-  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kFirst>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, 1);
+  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kFirst>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, 1);
   int set = 0;
   for (int k = 0; k + 1 < a.steps; ++k, set ^= 1)
-    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kMid>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, set);
-  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, T, kMuon, kLast>), grid, dim3(256), G::kLds, s, a, p, parts, part, ws, set);
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kMid>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
+  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kLast>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
 }
 
 // The path of a matrix by its sides: short side at most 64 with chunks of 64
 // columns where one holds the long side, else of 128; at most 128 with chunks of
-// 64; larger ones in tiles.
+// 64; larger ones in tiles.  Waves, measured with 4 / 8 / 16: 175 x 64 x 64
+// 20 / 15 / 15 us (4 000 of them 176 / 156 / 180), a step of 51 x 1088
+// 10.4 / 7.8 / 7.2, of 128 x 1000 35 / 22 / 20.
 enum { kThinSmall, kThin64, kThin128, kTiled };
+constexpr int kWavesSmall = 8, kWaves64 = 16, kWaves128 = 16;
 int path_of(int64_t rows, int64_t cols) {
   const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
   if (m <= 64) return n <= 64 ? kThinSmall : kThin64;
@@ -801,9 +800,9 @@ void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
 template <int T, bool kMuon>
 void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
   switch (path_of(a.rows, a.cols)) {
-    case kThinSmall: return launch_thin<2, 2, T, kMuon>(a, workspace, s);
-    case kThin64: return launch_thin<2, 4, T, kMuon>(a, workspace, s);
-    case kThin128: return launch_thin<4, 2, T, kMuon>(a, workspace, s);
+    case kThinSmall: return launch_thin<2, 2, kWavesSmall, T, kMuon>(a, workspace, s);
+    case kThin64: return launch_thin<2, 4, kWaves64, T, kMuon>(a, workspace, s);
+    case kThin128: return launch_thin<4, 2, kWaves128, T, kMuon>(a, workspace, s);
   }
   const NsPlan p = make_plan(a.rows, a.cols);
   double* part = (double*)workspace;
@@ -855,9 +854,9 @@ int64_t ns_workspace(int64_t batch, int64_t rows, int64_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
   int64_t stride = 0;
   switch (path_of(rows, cols)) {
-    case kThinSmall: stride = make_thin<2, 2>(rows, cols).stride; break;
-    case kThin64: stride = make_thin<2, 4>(rows, cols).stride; break;
-    case kThin128: stride = make_thin<4, 2>(rows, cols).stride; break;
+    case kThinSmall: stride = make_thin<2, 2, kWavesSmall>(rows, cols).stride; break;
+    case kThin64: stride = make_thin<2, 4, kWaves64>(rows, cols).stride; break;
+    case kThin128: stride = make_thin<4, 2, kWaves128>(rows, cols).stride; break;
     default: stride = make_plan(rows, cols).stride;
   }
   return batch * (kNormParts * 8 + stride);

@@ -83,12 +83,24 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _workspace(size_of, a: int, b: int, c: int, device) -> torch.Tensor:
-    """Scratch memory of a call from torch's allocator, which knows the stream."""
-    n = size_of(a, b, c)
-    if n < 0:
-        _check(n)
-    return torch.empty(n, dtype=torch.uint8, device=device)
+_sizes = {}
+
+
+def _workspace(name: str, a: int, b: int, c: int, device):
+    """Scratch memory of a call from torch's allocator, which knows the stream: (tensor, address, bytes).
+    The sizes are remembered: they depend on nothing but the numbers."""
+    key = (name, a, b, c)
+    n = _sizes.get(key)
+    if n is None:
+        n = getattr(_library(), name)(a, b, c)
+        if n < 0:
+            _check(n)
+        if len(_sizes) < 4096:
+            _sizes[key] = n
+    if n == 0:
+        return None, None, 0
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), n
 
 
 _coefficients = {}
@@ -126,9 +138,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
         _expect(out.shape == g.shape and out.dtype == g.dtype, "out differs from g in shape or type")
     _, _, _, ob, orow = _matrices(out, "out")
     lib, device = _library(), g.device.index
-    ws = _workspace(lib.lcn_orthogonalize_workspace, n, r, c, g.device)
+    ws, ws_ptr, ws_bytes = _workspace("lcn_orthogonalize_workspace", n, r, c, g.device)
     _check(lib.lcn_orthogonalize(device, _stream(device), dt, n, r, c, g.data_ptr(), sb, sr, out.data_ptr(),
-                                 ob, orow, int(steps), _triple(coefficients), eps, ws.data_ptr(), ws.numel()))
+                                 ob, orow, int(steps), _triple(coefficients), eps, ws_ptr, ws_bytes))
     return out
 
 
@@ -163,11 +175,10 @@ def muon_update(param: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor,
     if scale is None:
         scale = 0.2 * math.sqrt(max(r, c))
     lib, device = _library(), param.device.index
-    ws = _workspace(lib.lcn_orthogonalize_workspace, n, r, c, param.device)
+    ws, ws_ptr, ws_bytes = _workspace("lcn_orthogonalize_workspace", n, r, c, param.device)
     _check(lib.lcn_muon_update(device, _stream(device), dt, n, r, c, param.data_ptr(), pb, pr,
                                momentum.data_ptr(), mb, mr, grad.data_ptr(), gb, gr, lr_value, lr_ptr, scale, beta,
-                               int(nesterov), weight_decay, int(steps), _triple(coefficients), eps, ws.data_ptr(),
-                               ws.numel()))
+                               int(nesterov), weight_decay, int(steps), _triple(coefficients), eps, ws_ptr, ws_bytes))
 
 
 def quantize_weight(w: torch.Tensor, *, channel_dim: int = 0):
@@ -229,10 +240,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias
         _expect(n <= 1 or out.stride(-1) == 1, "out's last dimension is not contiguous")
         out2 = out if out.dim() == 2 else _rows(out, "out")
     lib, device = _library(), dev.index
-    ws = _workspace(lib.lcn_int8_linear_workspace, tokens, k, n, dev)
+    ws, ws_ptr, ws_bytes = _workspace("lcn_int8_linear_workspace", tokens, k, n, dev)
     _check(lib.lcn_int8_linear(device, _stream(device), dt, tokens, k, n, x2.data_ptr(), x2.stride(0), weight.data_ptr(),
-                               ws_row, scale.data_ptr(), bias_ptr, out2.data_ptr(), out2.stride(0), ws.data_ptr(),
-                               ws.numel()))
+                               ws_row, scale.data_ptr(), bias_ptr, out2.data_ptr(), out2.stride(0), ws_ptr, ws_bytes))
     return out
 
 
