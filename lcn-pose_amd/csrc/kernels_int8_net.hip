@@ -125,11 +125,15 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const WPrepHidden* __
   };
   float top = 0.f;
   bool bad = false;
-  for (int e = beg; e < end; ++e) {
-    float4 v[4];
-    load(idx[e].y, v);
+  // the blocks of a slab four at a time: their loads in flight together
+  for (int e = beg; e < end; e += 4) {
+    float4 v[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) see4(v[i], top, bad);
+    for (int u = 0; u < 4; ++u) load(idx[min(e + u, end - 1)].y, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) see4(v[u][i], top, bad);
   }
   tops[part][n] = top;
   bads[part][n] = bad;
@@ -139,14 +143,22 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const WPrepHidden* __
   for (int i = 0; i < 4; ++i) { top = fmaxf(top, tops[i][n]); anybad |= bads[i][n]; }
   const float factor = !anybad && top >= kTiny ? 127.f / top : 0.f;
   if (part == 0) ws[blockIdx.y * H + so * 64 + n] = anybad ? __builtin_nanf("") : top >= kTiny ? top / 127.f : 0.f;
-  for (int e = beg; e < end; ++e) {
-    const int blk = idx[e].y;
-    float4 v[4];
-    load(blk, v);
-    unsigned d[4];
+  for (int e = beg; e < end; e += 4) {
+    float4 v[4][4];
+    int blk[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = quant4(v[i], factor, anybad != 0);
-    *(v4u*)(out + (int64_t)blk * 4096 + n * 64 + part * 16) = v4u{d[0], d[1], d[2], d[3]};
+    for (int u = 0; u < 4; ++u) {
+      blk[u] = idx[min(e + u, end - 1)].y;
+      load(blk[u], v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (e + u >= end) break;
+      unsigned d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = quant4(v[u][i], factor, anybad != 0);
+      *(v4u*)(out + (int64_t)blk[u] * 4096 + n * 64 + part * 16) = v4u{d[0], d[1], d[2], d[3]};
+    }
   }
 }
 

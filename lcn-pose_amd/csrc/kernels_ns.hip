@@ -360,19 +360,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       if constexpr (MODE == kFinal) {
         const bool tall = a.rows > a.cols;
         const int j = rbj * 32 + l31;
-        if (j < pl.n) {
+        if (j >= pl.n) continue;
+        int64_t o[16];
+        float W[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int i = rbi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (i >= pl.m) continue;
-            const int64_t o = (int64_t)mat * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j);
-            if (a.momentum.p) {
-              float* W = (float*)a.out.p + o;
-              *W = fmaf(-lr * a.scale, v[e], *W * (1.f - lr * a.decay));
-            } else {
-              op_store<T>(a.out.p, o, v[e]);
-            }
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int i = rbi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+          o[e] = i < pl.m ? (int64_t)mat * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j) : -1;
+          if (a.momentum.p) W[e] = o[e] >= 0 ? ((const float*)a.out.p)[o[e]] : 0.f;  // all in flight before the first store
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (o[e] < 0) continue;
+          if (a.momentum.p) ((float*)a.out.p)[o[e]] = fmaf(-lr * a.scale, v[e], W[e] * (1.f - lr * a.decay));
+          else op_store<T>(a.out.p, o[e], v[e]);
         }
       } else {
         char* Y = g.Y + mat * g.stride + at;
@@ -613,17 +614,16 @@ __global__ __launch_bounds__(64 * NW) void ns_thin_kernel(NsArgs a, ThinPlan p, 
       for (int k = 0; k < G::XB; ++k) {
         const int t = w + NW * k, i0 = 16 * (t % G::MT) + 4 * l4, j = ch * W + 16 * (t / G::MT) + l15;
         if (j >= p.n) continue;
+        const int64_t o0 = b * a.out.batch + (tall ? (int64_t)j * a.out.row + i0 : (int64_t)i0 * a.out.row + j), step = tall ? 1 : a.out.row;
+        float W[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (kMuon && i0 + e < p.m) W[e] = ((const float*)a.out.p)[o0 + e * step];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int i = i0 + e;
-          if (i >= p.m) continue;
-          const int64_t o = b * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j);
-          if constexpr (kMuon) {
-            float* P = (float*)a.out.p + o;
-            *P = fmaf(-lr * a.scale, v[k][e], *P * (1.f - lr * a.decay));
-          } else {
-            op_store<T>(a.out.p, o, v[k][e]);
-          }
+          if (i0 + e >= p.m) continue;
+          if constexpr (kMuon) ((float*)a.out.p)[o0 + e * step] = fmaf(-lr * a.scale, v[k][e], W[e] * (1.f - lr * a.decay));
+          else op_store<T>(a.out.p, o0 + e * step, v[k][e]);
         }
       }
       return;
