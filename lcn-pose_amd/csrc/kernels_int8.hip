@@ -25,6 +25,7 @@ __host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64;
 __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 256; }
 
 constexpr int64_t kPanelTokens = 1024;
+constexpr int64_t kSlabTokens = 16384;  // one workgroup of 64 a CU
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
 
 // the factor 127 / top of a row and its scale, from the largest magnitude
@@ -37,13 +38,22 @@ __device__ __forceinline__ int quant(float v, float factor) {
   return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
+// four elements' integers as bytes; |v factor| <= 127 (1 + 2^-22), which rounds to 127:
+// no clamp.  Adding 1.5 2^23 rounds to the nearest integer, ties to even, like rint,
+// and leaves it in the low bits.
+__device__ __forceinline__ unsigned quant4(float a, float b, float c, float d, float factor, bool bad) {
+#pragma clang fp contract(off)  // the product is rounded before the sum
+  constexpr float kRound = 12582912.f;
+  const float qa = a * factor + kRound, qb = b * factor + kRound, qc = c * factor + kRound, qd = d * factor + kRound;
+  const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(qb), __float_as_uint(qa), 0x0c0c0400);
+  const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(qd), __float_as_uint(qc), 0x04000c0c);
+  return bad ? 0u : lo | hi;
+}
+
 // 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
 template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
-// (kOnce: not kept in the caches, which then hold the integers for the product)
-template <int T, bool kOnce>
-__device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {
-  const v4u* at = (const v4u*)((const char*)p + e * (16 / kVec<T>));
-  const v4u u = kOnce ? __builtin_nontemporal_load(at) : *at;
+template <int T>
+__device__ __forceinline__ void unpack_vec(v4u u, float (&v)[kVec<T>]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (T == kOpF32) v[i] = __uint_as_float(u[i]);
@@ -53,6 +63,12 @@ __device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kV
       v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
     }
   }
+}
+// (kOnce: not kept in the caches, which then hold the integers for the product)
+template <int T, bool kOnce>
+__device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {
+  const v4u* at = (const v4u*)((const char*)p + e * (16 / kVec<T>));
+  unpack_vec<T>(kOnce ? __builtin_nontemporal_load(at) : *at, v);
 }
 // largest magnitude of a wave's values, and whether one is an infinity or a NaN
 __device__ __forceinline__ void wave_top(float& top, bool& bad) {
@@ -110,11 +126,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
     auto put = [&](int c, const float (&v)[V]) {
       unsigned w[V / 4];
 #pragma unroll
-      for (int d = 0; d < V / 4; ++d) {
-        w[d] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[d] |= (bad ? 0u : (unsigned)(quant(v[4 * d + e], factor) & 255)) << (8 * e);
-      }
+      for (int d = 0; d < V / 4; ++d) w[d] = quant4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3], factor, bad);
       int8_t* o = out + (c * V >> 6) * panel + (c * V & 63);
       if constexpr (V == 4) *(unsigned*)o = w[0];
       else *(uint2*)o = make_uint2(w[0], w[1]);
@@ -296,7 +308,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
   // Row offsets are scalar: a store costs no address arithmetic.
   constexpr int kOut = T == kOpF32 ? 4 : 2;
   const int64_t obytes = ((int64_t)(trows - 1) * g.out_row + nrows) * kOut;
-  const bool near = obytes < 0x7fffffff;
+  const bool near = (int64_t)(64 * BI) * g.out_row * kOut + nrows * kOut < 0x7fffffff;  // no offset wraps, dropped rows' neither
   const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((char*)g.out + (t0 * g.out_row + n0) * kOut, 0, (int)obytes, 0x00020000);
 #pragma unroll
   for (int y = 0; y < BJ; ++y) {
@@ -325,6 +337,229 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
           }
         }
       }
+  }
+#endif
+}
+
+// ---- many tokens of moderate length ----------------------------------------------------------
+// A workgroup quantises 64 tokens into LDS and multiplies them by every channel:
+// x is read once, and no integers go through memory.  The integers lie as the
+// matrix instruction reads them: unit u (16 of K) of token r at block (u / 2,
+// r / 32), half u % 2, slot (r ^ u) % 32 of 16 bytes, so that 64 lanes write (16
+// units of one row) and read (32 rows of two units) all banks evenly.  Weights lie
+// the same way without the permutation, 1 KB a load, straight from L2 into
+// registers, four panels of 64 ahead.  A wave takes 64 channels at a time and runs
+// alone after the one barrier; two workgroups share a CU, so one's loads of x run
+// under the other's products.
+// Against the integers through memory (quantise, lay out, multiply), K 1088:
+// 65 536 tokens x 1088 channels 182 -> 160 us (fp32), 163 -> 130 (bf16); x 4352
+// channels 618 -> 465, 552 -> 377; 16 384 x 1088 60 -> 53, 59 -> 49; 8192 x 1088,
+// where half the CUs would have no workgroup, 39 -> 52: taken from one workgroup a
+// CU on.  What is left against the bytes' time (110 us) is the first workgroups'
+// loads, under which nothing runs yet.
+constexpr int kSlab = 64;                   // tokens
+constexpr int kSlabLds = 80 * 1024 - 512;   // half a CU's
+
+__global__ __launch_bounds__(256) void fragments_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int kp, int8_t* __restrict__ out) {
+  const int c = blockIdx.x * 16 + (threadIdx.x >> 4);  // channel, up to n rounded up to 64
+  const int k0 = blockIdx.y * 64 + (threadIdx.x & 15) * 4;
+  const int8_t* src = w + (int64_t)c * w_row + k0;
+  unsigned v = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c < n && k0 + e < k) v |= (unsigned)(uint8_t)src[e] << (8 * e);
+  *(unsigned*)(out + (int64_t)(c >> 5) * kp * 32 + (k0 >> 5) * 1024 + ((k0 >> 4) & 1) * 512 + (c & 31) * 16 + (k0 & 15)) = v;
+}
+
+template <int T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void int8_slab64_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ __attribute__((aligned(16))) float qs[kSlab];
+  const int64_t t0 = (int64_t)blockIdx.x * kSlab;
+  const int trows = (int)min((int64_t)kSlab, g.tokens - t0);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, l31 = lane & 31;
+  const int nk = (int)(g.kp / 64), tiles = (g.n + 63) / 64;
+  // weights: panel p of tile t, block y, half kk at ((2 t + y) 2 nk + 2 p + kk) KB
+  const int first = (w + blockIdx.x) & 3;  // the waves with a tile more change from workgroup to workgroup
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)g.w, 0, (int)g.w_bytes, 0x00020000);
+  struct Panel { v4i v[2][2]; };
+  int lt = first, lp = 0;
+  auto weights = [&](Panel& b) {
+    const int at = lt < tiles ? (lt * 4 * nk + 2 * lp) * 1024 : 0;  // (past the last tile: not used)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        b.v[y][kk] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, lane * 16, at + (y * 2 * nk + kk) * 1024, 0));
+    if (++lp == nk) { lp = 0; lt += 4; }
+  };
+  {
+    // four groups of four rows a wave, the next group's loads in flight
+    constexpr int V = kVec<T>, kRegs = T == kOpF32 ? 5 : 3, kRows = 4;
+    const int pieces = k / V, padded = (int)(g.kp / V);
+    struct Rows { v4u u[kRows][kRegs]; };
+    auto load = [&](int r0, Rows& m) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          m.u[j][i] = v4u{0, 0, 0, 0};
+          if (lane + 64 * i < pieces)
+            m.u[j][i] = __builtin_nontemporal_load((const v4u*)((const char*)x + (t0 + min(r0 + j, trows - 1)) * x_row * (16 / V) + (lane + 64 * i) * 16));
+        }
+    };
+    auto quantise = [&](int r0, const Rows& m) {
+      float top[kRows];
+      bool bad[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        top[j] = 0.f;
+        bad[j] = false;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          float v[V];
+          unpack_vec<T>(m.u[j][i], v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) see(v[e], top[j], bad[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) wave_top(top[j], bad[j]);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int r = r0 + j;
+        float factor, s;
+        row_scale(top[j], bad[j], factor, s);
+        if (lane == 0) qs[r] = s;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          const int at = (lane + 64 * i) * V, u = at >> 4;
+          if (lane + 64 * i < padded) {
+            float v[V];
+            unpack_vec<T>(m.u[j][i], v);
+            char* p = lds + (u >> 1) * 2048 + (r >> 5) * 1024 + (u & 1) * 512 + ((r ^ u) & 31) * 16 + (at & 15);
+            if constexpr (V == 4) *(unsigned*)p = quant4(v[0], v[1], v[2], v[3], factor, bad[j]);
+            else *(uint2*)p = make_uint2(quant4(v[0], v[1], v[2], v[3], factor, bad[j]), quant4(v[4], v[5], v[6], v[7], factor, bad[j]));
+          }
+        }
+      }
+    };
+    Rows m0, m1;
+    const int r0 = w * 16;
+    load(r0, m0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(r0 + 4, m1);
+    __builtin_amdgcn_sched_barrier(0);
+    quantise(r0, m0);
+    load(r0 + 8, m0);
+    __builtin_amdgcn_sched_barrier(0);
+    quantise(r0 + 4, m1);
+    load(r0 + 12, m1);
+    __builtin_amdgcn_sched_barrier(0);
+    quantise(r0 + 8, m0);
+    quantise(r0 + 12, m1);
+  }
+  Panel b0, b1, b2, b3;
+  const int total = (tiles - first + 3) / 4 * nk;  // panels of this wave (none: first >= tiles)
+  if (first < tiles) {
+    weights(b0);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(b1);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(b2);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(b3);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  if (first >= tiles) return;
+  v16i acc[2][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  };
+  clear();
+  constexpr int kOut = T == kOpF32 ? 4 : 2;
+  const int64_t obytes = ((int64_t)(trows - 1) * g.out_row + g.n) * kOut;
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((char*)g.out + t0 * g.out_row * kOut, 0, (int)obytes, 0x00020000);
+  int tile = first;
+  float scales[2], biases[2];  // of this tile's channels
+  const float* bias = g.bias ? g.bias : g.ws;  // (read without a branch, whose merge would wait for the loads in flight)
+  auto channels = [&]() {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int c = min(tile * 64 + y * 32 + l31, g.n - 1);
+      scales[y] = g.ws[c];
+      biases[y] = bias[c];
+    }
+  };
+  channels();
+  auto finish = [&]() {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int c = tile * 64 + y * 32 + l31;
+      const bool in = c < g.n;
+      const float sw = scales[y], b = g.bias ? biases[y] : 0.f;
+      const int vout = in ? (4 * h * (int)g.out_row + c) * kOut : -1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = i * 32 + 8 * q;
+          const float4 s4 = *(const float4*)(qs + r + 4 * h);
+          const float se[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = (float)acc[i][y][4 * q + e] * se[e] * sw + b;
+            const int so = (r + e) * (int)g.out_row * kOut;
+            if constexpr (T == kOpF32) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), ro, vout, so, 0);
+            else if constexpr (T == kOpBF16) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), ro, vout, so, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (_Float16)v), ro, vout, so, 0);
+          }
+        }
+    }
+    clear();
+    tile += 4;
+    channels();
+  };
+  struct Frag { v4i v[2][2]; };
+  auto fetch = [&](int p, Frag& f) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int u = 4 * p + 2 * kk + h;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f.v[kk][i] = *(const v4i*)(lds + (2 * p + kk) * 2048 + i * 1024 + h * 512 + ((l31 ^ u) & 31) * 16);
+    }
+  };
+  Frag f0, f1;
+  int p = 0;
+  fetch(0, f0);
+  auto step = [&](Panel& b, Frag& f, Frag& next) {
+    const int after = p + 1 == nk ? 0 : p + 1;
+    fetch(after, next);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) acc[i][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.v[kk][i], b.v[y][kk], acc[i][y], 0, 0, 0);
+    weights(b);
+    if (after == 0 && tile < tiles) finish();
+    p = after;
+  };
+  // (one exit, or the compiler waits for all loads at the top; panels past the last are multiplied and dropped)
+  for (int s = 0; s < total; s += 4) {
+    step(b0, f0, f1);
+    step(b1, f1, f0);
+    step(b2, f0, f1);
+    step(b3, f1, f0);
   }
 #endif
 }
@@ -509,6 +744,17 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
     }
     return;
   }
+  // Many rows of whole 16-byte pieces, two workgroups' integers in a CU's LDS (K up to 1216), 32-bit offsets.
+  constexpr int V = kVec<T>;
+  const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && a.x_row % V == 0;
+  const int64_t n64 = pad64(a.n);
+  if (a.tokens >= kSlabTokens && al && kp * kSlab <= kSlabLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
+    hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, wp);
+    g.w = wp;
+    g.w_bytes = n64 * kp;
+    hipLaunchKernelGGL((int8_slab64_kernel<T>), dim3((unsigned)((a.tokens + kSlab - 1) / kSlab)), dim3(256), (unsigned)(kp * kSlab), s, g, a.x, a.x_row, a.k);
+    return;
+  }
   // The weights as panels where many token tiles read them, and where 16-byte
   // loads at 32-bit offsets cannot address their rows (k % 4: the loads' bounds
   // check drops a dword that ends past the last row).
@@ -541,7 +787,7 @@ int64_t int8_workspace(int64_t tokens, int64_t k, int64_t n) {
   if (tokens <= 0 || k <= 0 || n <= 0) return 0;
   if (fused(tokens, k)) return 0;
   const int64_t most = round_tokens(tokens, k);
-  return pad256(most * 4) + pad256(most * pad64(k)) + pad256(n * pad64(k));
+  return pad256(most * 4) + pad256(most * pad64(k)) + pad256(pad64(n) * pad64(k));
 }
 
 void launch_int8(const Int8Args& a, void* workspace, hipStream_t s) {

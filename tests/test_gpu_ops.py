@@ -267,6 +267,36 @@ def test_int8_linear_shapes(t, k, n, dtype):
         int8_close(y, x, w, s, b)
 
 
+# many tokens: 64 at a time are quantised next to their product while K fits (1216), panels through memory past that
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,k,n", [(16384, 1088, 1088), (16447, 64, 64), (16385, 1216, 129), (17001, 80, 1), (16400, 8, 300),
+                                   (20000, 320, 200), (16384, 1280, 257), (16401, 1003, 96), (16383, 136, 449)])
+def test_int8_linear_many_tokens(t, k, n, dtype):
+    x, w, s, b = int8_case(t, k, n, dtype, seed=t + k)
+    wide = torch.full((t + 3, n + 5), 7.0, device="cuda", dtype=dtype)
+    got = ops.int8_linear(x, w, s, b, out=wide[1:t + 1, 2:n + 2])
+    int8_close(got, x, w, s, b)
+    wide[1:t + 1, 2:n + 2] = 7.0
+    assert bool((wide == 7.0).all())
+    x[5, k // 2] = float("nan")
+    x[8000] = 0
+    plain = ops.int8_linear(x, w, s)
+    assert bool(plain[5].isnan().all()) and bool((plain[8000] == 0).all()) and bool(plain[6:].isfinite().all())
+    assert torch.equal(plain[6:], ops.int8_linear(x, w, s)[6:])
+
+
+def test_int8_linear_rows_far_apart():
+    # 32 rows of the output span more than 2^31 bytes: offsets of the dropped rows of the last tile do not wrap
+    for t in (65, 1030):
+        x, w, s, b = int8_case(t, 48, 40, torch.float32, seed=3)
+        pitch = (1 << 25) if t == 65 else (1 << 23) + 64
+        store = torch.empty((t - 1) * pitch + 40, device="cuda")
+        out = store.as_strided((t, 40), (pitch, 1))
+        ops.int8_linear(x, w, s, b, out=out)
+        int8_close(out.clone(), x, w, s, b)
+        del store, out
+
+
 def test_int8_linear_long_k_and_extreme_integers():
     k = 131072
     x = torch.full((3, k), 2.0, device="cuda")
