@@ -269,10 +269,9 @@ int lcn_eval_mpjpe_static(int32_t device, int64_t n, const double* pred, const d
  * synchronise and may be captured into a graph.  Scratch memory is the
  * caller's: `workspace`, 256-byte aligned, at least as many bytes as the
  * matching _workspace function returns (negative: LCN_E_*; 0: none needed,
- * NULL will do); a workspace
- * belongs to one call at a time in stream order, so calls on two streams (or
- * two graphs that may run at once) need two.  dtype: LCN_DTYPE_F32, _BF16 or
- * _F16.  Matrices have a contiguous last dimension; strides are in elements
+ * NULL will do).  A workspace belongs to one call at a time in stream order, so
+ * calls on two streams (or two graphs that may run at once) need two.  dtype:
+ * LCN_DTYPE_F32, _BF16 or _F16.  Matrices have a contiguous last dimension; strides are in elements
  * and not negative; batch strides are unused with batch 1, row strides with one
  * row.  Operands that would overlap where they must not are LCN_E_ARG, an
  * empty batch is LCN_OK.  Errors: lcn_last_error(NULL).  No counterpart in the
@@ -295,8 +294,8 @@ int lcn_orthogonalize(int32_t device, void* stream, int32_t dtype, int64_t batch
 /* One Muon step on batch float32 matrices, in place:
  *   momentum <- beta momentum + grad;  u = grad + beta momentum (nesterov != 0) or momentum
  *   param <- (1 - lr weight_decay) param - lr scale NS(u)
- * lr_dev (device memory, one float) is read instead of lr when not NULL, so a
- * captured graph follows a schedule.  Workspace: lcn_orthogonalize_workspace. */
+ * lr_dev (device memory, one float, outside the operands) is read instead of lr
+ * when not NULL, so a captured graph follows a schedule.  Workspace: lcn_orthogonalize_workspace. */
 int lcn_muon_update(int32_t device, void* stream, int32_t grad_dtype, int64_t batch, int64_t rows, int64_t cols,
                     float* param, int64_t param_batch, int64_t param_row, float* momentum, int64_t momentum_batch,
                     int64_t momentum_row, const void* grad, int64_t grad_batch, int64_t grad_row, float lr,

@@ -25,30 +25,7 @@ __host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64;
 __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 256; }
 
 constexpr int64_t kPanelTokens = 1024;
-constexpr int64_t kSlabTokens = 16384;  // one workgroup of 64 a CU
-constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
-
-// the factor 127 / top of a row and its scale, from the largest magnitude
-__device__ __forceinline__ void row_scale(float top, bool bad, float& factor, float& scale) {
-  factor = !bad && top >= kTiny ? 127.f / top : 0.f;
-  scale = bad ? __builtin_nanf("") : top >= kTiny ? top / 127.f : 0.f;
-}
-__device__ __forceinline__ int quant(float v, float factor) {
-  const float r = rintf(v * factor);
-  return (int)fminf(fmaxf(r, -127.f), 127.f);
-}
-
-// four elements' integers as bytes; |v factor| <= 127 (1 + 2^-22), which rounds to 127:
-// no clamp.  Adding 1.5 2^23 rounds to the nearest integer, ties to even, like rint,
-// and leaves it in the low bits.
-__device__ __forceinline__ unsigned quant4(float a, float b, float c, float d, float factor, bool bad) {
-#pragma clang fp contract(off)  // the product is rounded before the sum
-  constexpr float kRound = 12582912.f;
-  const float qa = a * factor + kRound, qb = b * factor + kRound, qc = c * factor + kRound, qd = d * factor + kRound;
-  const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(qb), __float_as_uint(qa), 0x0c0c0400);
-  const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(qd), __float_as_uint(qc), 0x04000c0c);
-  return bad ? 0u : lo | hi;
-}
+constexpr int64_t kGroupTokens = 16384;  // one workgroup of 64 a CU
 
 // 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
 template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
@@ -152,8 +129,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
     row_scale(top, bad, factor, s);
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
-      if (64 * i < kp) out[i * panel + lane] = bad ? (int8_t)0 : (int8_t)quant(keep[i], factor);
-    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[(c >> 6) * panel + lane] = c < k && !bad ? (int8_t)quant(op_load<T>(x, r + c), factor) : (int8_t)0;
+      if (64 * i < kp) out[i * panel + lane] = bad ? (int8_t)0 : quant(keep[i], factor);
+    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[(c >> 6) * panel + lane] = c < k && !bad ? quant(op_load<T>(x, r + c), factor) : (int8_t)0;
   }
   if (lane == 0) scale[t] = s;
 }
@@ -357,8 +334,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void i
 // where half the CUs would have no workgroup, 39 -> 52: taken from one workgroup a
 // CU on.  What is left against the bytes' time (110 us) is the first workgroups'
 // loads, under which nothing runs yet.
-constexpr int kSlab = 64;                   // tokens
-constexpr int kSlabLds = 80 * 1024 - 512;   // half a CU's
+constexpr int kGroup = 64;                   // tokens
+constexpr int kGroupLds = 80 * 1024 - 512;   // half a CU's
 
 __global__ __launch_bounds__(256) void fragments_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int kp, int8_t* __restrict__ out) {
   const int c = blockIdx.x * 16 + (threadIdx.x >> 4);  // channel, up to n rounded up to 64
@@ -372,12 +349,12 @@ __global__ __launch_bounds__(256) void fragments_kernel(const int8_t* __restrict
 }
 
 template <int T>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void int8_slab64_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void int8_group_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
 #ifdef __HIP_DEVICE_COMPILE__
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ __attribute__((aligned(16))) float qs[kSlab];
-  const int64_t t0 = (int64_t)blockIdx.x * kSlab;
-  const int trows = (int)min((int64_t)kSlab, g.tokens - t0);
+  __shared__ __attribute__((aligned(16))) float qs[kGroup];
+  const int64_t t0 = (int64_t)blockIdx.x * kGroup;
+  const int trows = (int)min((int64_t)kGroup, g.tokens - t0);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l31 = lane & 31;
   const int nk = (int)(g.kp / 64), tiles = (g.n + 63) / 64;
@@ -629,9 +606,9 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
       if (at == 0) qs[t] = s;
 #pragma unroll
       for (int i = 0; i < kRegs; ++i)
-        if (at + i * step < kp) lds[t * pitch + at + i * step] = bad ? (char)0 : (char)quant(keep[i], factor);
+        if (at + i * step < kp) lds[t * pitch + at + i * step] = bad ? (char)0 : quant(keep[i], factor);
       for (int c = at + kRegs * step; c < kp; c += step)
-        lds[t * pitch + c] = c < k && !bad ? (char)quant(op_load<T>(x, t * x_row + c), factor) : (char)0;
+        lds[t * pitch + c] = c < k && !bad ? quant(op_load<T>(x, t * x_row + c), factor) : (char)0;
     }
     __syncthreads();
   } else if (threadIdx.x < tokens) {
@@ -684,7 +661,7 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWArgs a) {
   row_scale(top, bad, factor, s);
   if (lane == 0) a.scale[n] = s;
   for (int c = lane; c < a.k; c += 64)
-    a.q[(int64_t)n * a.k + c] = bad ? (int8_t)0 : (int8_t)quant(op_load<T>(a.w, n * a.w_n + c * a.w_k), factor);
+    a.q[(int64_t)n * a.k + c] = bad ? (int8_t)0 : quant(op_load<T>(a.w, n * a.w_n + c * a.w_k), factor);
 }
 
 template <int T>
@@ -748,11 +725,11 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
   constexpr int V = kVec<T>;
   const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && a.x_row % V == 0;
   const int64_t n64 = pad64(a.n);
-  if (a.tokens >= kSlabTokens && al && kp * kSlab <= kSlabLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
+  if (a.tokens >= kGroupTokens && al && kp * kGroup <= kGroupLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
     hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, wp);
     g.w = wp;
     g.w_bytes = n64 * kp;
-    hipLaunchKernelGGL((int8_slab64_kernel<T>), dim3((unsigned)((a.tokens + kSlab - 1) / kSlab)), dim3(256), (unsigned)(kp * kSlab), s, g, a.x, a.x_row, a.k);
+    hipLaunchKernelGGL((int8_group_kernel<T>), dim3((unsigned)((a.tokens + kGroup - 1) / kGroup)), dim3(256), (unsigned)(kp * kGroup), s, g, a.x, a.x_row, a.k);
     return;
   }
   // The weights as panels where many token tiles read them, and where 16-byte

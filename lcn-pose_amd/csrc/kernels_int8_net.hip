@@ -17,12 +17,6 @@ namespace lcn {
 
 namespace {
 
-constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100: rows below it count as zero
-
-__device__ __forceinline__ unsigned quant4(float4 v, float factor, bool bad) {
-  auto one = [&](float x) { return bad ? 0u : (unsigned)((int)fminf(fmaxf(rintf(x * factor), -127.f), 127.f) & 255); };
-  return one(v.x) | one(v.y) << 8 | one(v.z) << 16 | one(v.w) << 24;
-}
 __device__ __forceinline__ void see4(float4 v, float& top, bool& bad) {
   const float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
   bad |= !(fabsf(v.x) < __builtin_inff() && fabsf(v.y) < __builtin_inff() && fabsf(v.z) < __builtin_inff() && fabsf(v.w) < __builtin_inff());
@@ -78,12 +72,13 @@ __global__ __launch_bounds__(64 * kQuantWaves) void quant_tiles_kernel(const flo
 #pragma unroll
   for (int i = 0; i < kQuantWaves; ++i) { top = fmaxf(top, tops[i][row]); anybad |= bads[i][row]; }
   bad = anybad != 0;
-  const float factor = !bad && top >= kTiny ? 127.f / top : 0.f;
-  if (w == 0 && h == 0) qs[rt * 32 + row] = bad ? __builtin_nanf("") : top >= kTiny ? top / 127.f : 0.f;
+  float factor, scale_of;
+  row_scale(top, bad, factor, scale_of);
+  if (w == 0 && h == 0) qs[rt * 32 + row] = scale_of;
   auto put = [&](int si, const float4 (&v)[8]) {
     unsigned d[8];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) d[g] = quant4(v[g], factor, bad);
+    for (int g = 0; g < 8; ++g) d[g] = quant4(v[g].x, v[g].y, v[g].z, v[g].w, factor, bad);
     // features 8 g + 4 h .. of this lane and its partner (same row, other half):
     // half h stores bytes 32 h .. 32 h + 31 of the row
     unsigned o[8];
@@ -141,8 +136,9 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const WPrepHidden* __
   int anybad = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) { top = fmaxf(top, tops[i][n]); anybad |= bads[i][n]; }
-  const float factor = !anybad && top >= kTiny ? 127.f / top : 0.f;
-  if (part == 0) ws[blockIdx.y * H + so * 64 + n] = anybad ? __builtin_nanf("") : top >= kTiny ? top / 127.f : 0.f;
+  float factor, scale;
+  row_scale(top, anybad != 0, factor, scale);
+  if (part == 0) ws[blockIdx.y * H + so * 64 + n] = scale;
   for (int e = beg; e < end; e += 4) {
     float4 v[4][4];
     int blk[4];
@@ -156,7 +152,7 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const WPrepHidden* __
       if (e + u >= end) break;
       unsigned d[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = quant4(v[u][i], factor, anybad != 0);
+      for (int i = 0; i < 4; ++i) d[i] = quant4(v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w, factor, anybad != 0);
       *(v4u*)(out + (int64_t)blk[u] * 4096 + n * 64 + part * 16) = v4u{d[0], d[1], d[2], d[3]};
     }
   }

@@ -192,6 +192,10 @@ int lcn_muon_update(int32_t device, void* stream, int32_t grad_dtype, int64_t ba
   if (!writable(vp) || !writable(vm)) return fail(who, "the strides of the parameter or the momentum let elements overlap");
   if (!aligned(vp) || !aligned(vm) || !aligned(vg) || (uintptr_t)lr_dev % 4) return fail(who, "operand not aligned to its type");
   if (overlap(vp, vm) || overlap(vp, vg) || overlap(vm, vg)) return fail(who, "param, momentum and grad must not overlap");
+  if (lr_dev) {  // read while param and momentum are written
+    const View vl{lr_dev, 1, 1, 1, 0, 1, 4};
+    if (overlap(vp, vl) || overlap(vm, vl) || in_block(vl, workspace, workspace_bytes)) return fail(who, "lr_dev lies in an operand or the workspace");
+  }
   OP_CHECK(check_workspace(who, workspace, workspace_bytes, ns_workspace(batch, rows, cols)));
   if (in_block(vp, workspace, workspace_bytes) || in_block(vm, workspace, workspace_bytes) || in_block(vg, workspace, workspace_bytes))
     return fail(who, "the workspace overlaps an operand");

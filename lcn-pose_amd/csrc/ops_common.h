@@ -25,6 +25,28 @@ __device__ __forceinline__ void op_store(void* p, int64_t e, float v) {
   else ((_Float16*)p)[e] = (_Float16)v;
 }
 
+// ---- int8 quantisation of a row --------------------------------------------------------------
+constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100: a row below it counts as zero
+
+// the factor 127 / top of a row and its scale, from the largest magnitude
+__device__ __forceinline__ void row_scale(float top, bool bad, float& factor, float& scale) {
+  factor = !bad && top >= kTiny ? 127.f / top : 0.f;
+  scale = bad ? __builtin_nanf("") : top >= kTiny ? top / 127.f : 0.f;
+}
+// rint(v factor) in the low byte.  |v factor| <= 127 (1 + 2^-22), which rounds to
+// 127: no clamp.  Adding 1.5 2^23 rounds to the nearest integer, ties to even.
+__device__ __forceinline__ unsigned quant_bits(float v, float factor) {
+#pragma clang fp contract(off)  // the product is rounded before the sum
+  return __float_as_uint(v * factor + 12582912.f);
+}
+__device__ __forceinline__ int8_t quant(float v, float factor) { return (int8_t)quant_bits(v, factor); }
+// four integers as bytes, zeros for a bad row
+__device__ __forceinline__ unsigned quant4(float a, float b, float c, float d, float factor, bool bad) {
+  const unsigned lo = __builtin_amdgcn_perm(quant_bits(b, factor), quant_bits(a, factor), 0x0c0c0400);
+  const unsigned hi = __builtin_amdgcn_perm(quant_bits(d, factor), quant_bits(c, factor), 0x04000c0c);
+  return bad ? 0u : lo | hi;
+}
+
 // Waits until at most N of this wave's vector loads are outstanding and all its
 // LDS reads have returned, then for the other waves of the workgroup.  Nothing
 // that touches memory moves across.

@@ -61,6 +61,8 @@ def _tensor(t, name: str, device=None) -> torch.Tensor:
         raise ValueError(f"{name} is on {t.device}: these operators run on the GPU only")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view: call resolve_neg() on it")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad()")
     return t

@@ -225,6 +225,11 @@ def test_muon_refuses_on_the_gpu():
         ops.orthogonalize(p, coefficients=(1.0, 2.0))
     with pytest.raises(ValueError):
         ops.orthogonalize(p, out=p.half())
+    z = torch.randn(8, 16, device="cuda", dtype=torch.complex64)
+    negated = z.conj().imag  # the negation is a flag of the view
+    assert negated.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        ops.orthogonalize(negated)
 
 
 # ---- int8 ----------------------------------------------------------------------------------------
@@ -295,6 +300,26 @@ def test_int8_linear_rows_far_apart():
         ops.int8_linear(x, w, s, b, out=out)
         int8_close(out.clone(), x, w, s, b)
         del store, out
+
+
+@pytest.mark.parametrize("t,k,n", [(16500, 131072, 32), (2000100, 1088, 16)])
+def test_int8_linear_offsets_past_32_bits(t, k, n):
+    # three rounds of at most 1 GiB of integers; and 31 250 groups of 64 tokens in one launch
+    x = torch.empty(t, k, device="cuda", dtype=torch.float16).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    _, w, s, b = int8_case(1, k, n, torch.float16, seed=2)
+    s *= 1e-3  # sums of 131 072 products stay inside fp16's range
+    got = ops.int8_linear(x, w, s, b)
+    rows = [0, 63, 64, 8191, 8192, 8193, t // 2, 16383, 16384, t - 65, t - 2, t - 1]
+    int8_close(got[rows], x[rows], w, s, b)
+
+
+def test_orthogonalize_offsets_past_32_bits():
+    store = torch.empty((3 << 31) + 200 * 136, device="cuda", dtype=torch.bfloat16)
+    for shape in ((200, 136), (100, 136)):
+        g = store.as_strided((3,) + shape, (3 << 30, 136, 1))
+        g.copy_(gradient((3,) + shape, torch.bfloat16, 40))
+        want = ops.orthogonalize(g.contiguous())
+        assert torch.equal(ops.orthogonalize(g, out=g), want)
 
 
 def test_int8_linear_long_k_and_extreme_integers():

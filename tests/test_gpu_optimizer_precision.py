@@ -10,6 +10,7 @@ import torch
 
 import lcn_oracle as O
 from lcn_testutil import make_cfg, make_network, perturbed_params, synthetic_batch
+from test_gpu_multirank import ThreadAllReduce, run_ranks
 
 pytestmark = pytest.mark.gpu
 
@@ -169,6 +170,65 @@ def test_int8_hidden_layers(kw, batch):
     np.testing.assert_array_equal(net.get_params(), other.get_params())
     net.set_precision("fp32")
     np.testing.assert_array_equal(net.forward(x), other.forward(x))
+
+
+def test_muon_replicas_of_two_ranks_stay_equal():
+    """The update follows the all-reduced gradients: both ranks' weights and momenta are the same bits, and the
+    hidden weights move by the orthogonalised direction of the gradient the ranks report."""
+    cfg = make_cfg(F=64, L=1, knn=2)
+    theta = O.flatten(cfg, perturbed_params(cfg, seed=7))
+    x, lab = synthetic_batch(96, 2, seed=3)
+    ar = ThreadAllReduce(2)
+
+    def rank(r):
+        net = make_network(cfg, max_batch=64)
+        net.comm_init_host(r, 2, ar.for_rank(r))
+        net.set_optimizer("muon", momentum=0.9)
+        net.set_params(theta)
+        part = slice(0, 40) if r == 0 else slice(40, 96)
+        lr = net.train_step(x[part], lab[part], update=False, keep_grads=True)[1]
+        grads = net.get_grads()
+        net.train_step(x[part], lab[part])
+        first = net.get_params()
+        net.train_step(x[part], lab[part])
+        out = grads, first, net.get_params(), net.get_optimizer_state()[0], lr, hidden(net)
+        net.close()
+        return out
+
+    one, two = run_ranks(2, rank)
+    for a, b in zip(one[:4], two[:4]):
+        np.testing.assert_array_equal(a, b)
+    grads, first, _, _, lr, names = one
+    for n, off, shape in names:
+        sl = slice(off, off + shape[0] * shape[1])
+        o = newton_schulz(1.9 * grads[sl].reshape(shape).astype(np.float64))   # g + 0.9 g, at any scale
+        want = theta[sl].reshape(shape) - lr * 0.2 * math.sqrt(1088) * o
+        # as above: the direction's error, then the parameter's roundings
+        bound = lr * 0.2 * math.sqrt(1088) * np.linalg.norm(o) * 2.0 ** -20 * MUON[0] ** 5 + 3 * 2.0 ** -24 * np.linalg.norm(want)
+        assert np.linalg.norm(first[sl].reshape(shape) - want) <= bound
+
+
+def test_int8_poses_of_two_ranks():
+    """Without batch statistics a pose's prediction depends on nothing but the pose."""
+    cfg = make_cfg(F=64, L=1, knn=2, batch_norm=False)
+    theta = O.flatten(cfg, perturbed_params(cfg, seed=8))
+    x, _ = synthetic_batch(96, 2, seed=4)
+    ar = ThreadAllReduce(2)
+
+    def rank(r):
+        net = make_network(cfg, max_batch=64)
+        net.comm_init_host(r, 2, ar.for_rank(r))
+        net.set_params(theta)
+        net.set_precision("int8")
+        out = net.forward(x[:40] if r == 0 else x[40:])
+        net.close()
+        return out
+
+    parts = run_ranks(2, rank)
+    whole = make_network(cfg, max_batch=96)
+    whole.set_params(theta)
+    whole.set_precision("int8")
+    np.testing.assert_array_equal(np.concatenate(parts), whole.forward(x))
 
 
 def test_int8_predict_dataset_and_repeats():

@@ -69,6 +69,7 @@ def _muon(lib, **kw):
     (dict(beta=float("nan")), "beta"), (dict(p=None), "null"), (dict(m=None), "null"), (dict(g=None), "null"),
     (dict(p=B), "must not overlap"), (dict(g=A), "must not overlap"), (dict(g=B + 4), "must not overlap"),
     (dict(pr=8), "overlap"), (dict(mb=0), "overlap"), (dict(gr=-1), "gradient"), (dict(lr_dev=A + 2), "aligned"),
+    (dict(lr_dev=A + 64), "lr_dev"), (dict(lr_dev=B), "lr_dev"), (dict(lr_dev=WS + 256), "lr_dev"),
     (dict(m=WS), "workspace overlaps"), (dict(wsb=0), "needed"), (dict(steps=-1), "steps"),
 ])
 def test_muon_update_refuses(lib, kw, word):
