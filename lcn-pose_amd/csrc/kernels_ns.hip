@@ -191,19 +191,20 @@ struct NsProd {
 #define NS_LDS(SRC, VOFF, SOFF, DST) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(SRC, (__attribute__((address_space(3))) void*)(DST), 16, VOFF, SOFF, 0, 0)
 
-// One tile of D = P Q^T with sides of 64 NB, four waves of 32 NB x 32 NB blocks;
-// K in steps of 16 (NB 2) or 32 (NB 1) through a ring of four LDS buffers filled by
-// LDS-DMA (16 KB a stage: hi and lo of both operands), three to four stages in
-// flight (eight buffers measured the same, two 20 us for 12 where CUs are idle): with one stage in flight a
-// lone workgroup of a CU spent three quarters of its time waiting for the next
-// (46 us for six 1088 x 1088 Gram matrices).  The buffers are LDS objects of their own, and
-// a stage's object is known at compile time, so the compiler adds no waits of
-// its own for loads into the others.
-template <int MODE, int T, int NB>
+// One tile of D = P Q^T of 64 NI x 64 NJ, four waves of 32 NI x 32 NJ; K in steps of
+// 16 (64 x 64: 32) through a ring of four LDS buffers filled by LDS-DMA (16 KB a
+// stage, 12 KB for 128 x 64: hi and lo of both operands), three to four stages in
+// flight (eight buffers measured the same, two 20 us for 12 where CUs are idle):
+// with one stage in flight a lone workgroup of a CU spent three quarters of its
+// time waiting for the next (46 us for six 1088 x 1088 Gram matrices).  The
+// buffers are LDS objects of their own, and a stage's object is known at compile
+// time, so the compiler adds no waits of its own for loads into the others.
+template <int MODE, int T, int NI, int NJ>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void ns_prod_kernel(NsProd g, NsArgs a, NsPlan pl) {
-  constexpr int R = 4, L = 4;  // ring buffers, loads of a wave per stage
-  constexpr int KK = 2 / NB, TB = 2 * NB;  // 16-wide pieces of K a stage, row blocks of a tile's side
-  __shared__ __attribute__((aligned(16))) char l0[16384], l1[16384], l2[16384], l3[16384];
+  constexpr int KK = 2 / NI, TI = 2 * NI, TJ = 2 * NJ;  // 16-wide pieces of K a stage, row blocks of a tile's sides
+  constexpr int kP = TI * KK * 1024, kQ = TJ * KK * 1024, kStage = 2 * (kP + kQ);  // bytes of a plane's part of a stage
+  constexpr int R = 4, L = kStage / 4096;  // ring buffers, loads of a wave per stage
+  __shared__ __attribute__((aligned(16))) char l0[kStage], l1[kStage], l2[kStage], l3[kStage];
 #define NS_BUF(I) ((I) % R == 0 ? l0 : (I) % R == 1 ? l1 : (I) % R == 2 ? l2 : l3)
   // The whole tiles of all matrices come first, then those with fewer row blocks
   // of either operand.
@@ -213,7 +214,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const int mat = id / (rest ? g.rest : g.whole);
   int t = id - mat * (rest ? g.rest : g.whole);
   int ti, tj;
-  if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle, ti >= tj, row after row
+  if constexpr (NI != NJ) {
+    // symmetric: pairs of 64-row blocks ti with the columns up to theirs, then, if
+    // the number of blocks is odd, all rows with the last block's columns
+    if (rest) {
+      ti = t;
+      tj = 2 * g.ti;
+    } else {
+      ti = (int)((sqrtf(4.f * t + 1.f) - 1.f) * 0.5f);
+      while (ti * (ti + 1) > t) --ti;
+      while ((ti + 1) * (ti + 2) <= t) ++ti;
+      tj = t - ti * (ti + 1);
+    }
+  } else if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle, ti >= tj, row after row
     if (rest) t += g.whole;
     ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > t) --ti;
@@ -223,7 +236,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     ti = t % g.ti;
     tj = t / g.ti;
   } else {  // the last column of tiles, if partial, then the last row
-    const int side = g.Rq / 32 > g.tj * TB ? g.ti : 0;
+    const int side = g.Rq / 32 > g.tj * TJ ? g.ti : 0;
     ti = t < side ? t : g.ti;
     tj = t < side ? g.tj : t - side;
   }
@@ -232,41 +245,43 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const char* Pm = g.P + mat * g.stride;
   const char* Qm = g.Q + mat * g.stride;
   const int nPb = g.Rp / 32, nQb = g.Rq / 32;
-  // this wave stages one row block (NB 1: one 16-wide piece of it) of both operand
-  // tiles (a block past the end repeats the last one; its results are not stored)
-  const int sb = NB == 2 ? w : w >> 1, sk = NB == 2 ? 0 : (w & 1) * 1024;
+  // this wave stages one row block (64 x 64: one 16-wide piece of it) of both operand
+  // tiles (128 x 64: of one half of Q's; a block past the end repeats the last one,
+  // its results are not stored)
+  const int sb = NI == 2 ? w : w >> 1, sk = NI == 2 ? 0 : (w & 1) * 1024;
   const int rb_bytes = g.K * 64;
-  const int pb = min(ti * TB + sb, nPb - 1), qb = min(tj * TB + sb, nQb - 1);
+  const int pb = min(ti * TI + sb, nPb - 1), qb = min(tj * TJ + (NI == NJ ? sb : w & 1), nQb - 1);
   const __amdgpu_buffer_rsrc_t rph = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rpl = __builtin_amdgcn_make_buffer_rsrc((void*)(Pm + g.p_lo + (int64_t)pb * rb_bytes), 0, rb_bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rqh = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + (NI != NJ && w >= 2 ? g.q_lo : 0) + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
-  // stage layout: P hi | P lo | Q hi | Q lo, 4 KB each = row blocks x 1 KB pieces of K
+  // stage layout: P hi | P lo | Q hi | Q lo, row blocks x 1 KB pieces of K
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
     const int so = ks * (1024 * KK) + sk;
     NS_LDS(rph, vo, so, d);
-    NS_LDS(rpl, vo, so, d + 4096);
-    NS_LDS(rqh, vo, so, d + 8192);
-    NS_LDS(rql, vo, so, d + 12288);
+    NS_LDS(rpl, vo, so, d + kP);
+    NS_LDS(rqh, vo, so, d + 2 * kP);
+    if constexpr (NI == NJ) NS_LDS(rql, vo, so, d + 2 * kP + kQ);
   };
-  f32x16 acc[NB][NB] = {}, cr = {};  // cr: NB 1 alternates between two sums, which do not wait for each other
+  f32x16 acc[NI][NJ] = {}, cr = {};  // cr: 64 x 64 alternates between two sums, which do not wait for each other
   const int nk = g.K / (16 * KK);
-  struct Frag { half8 ph[NB * KK], pl[NB * KK], qh[NB * KK], ql[NB * KK]; };  // [row block][piece of K]
+  struct Frag { half8 ph[NI * KK], pl[NI * KK], qh[NJ * KK], ql[NJ * KK]; };  // [row block][piece of K]
   auto fetch = [&](const char* buf, Frag& f) {
+    const char *p = buf + wi * NI * KK * 1024 + vo, *q = buf + 2 * kP + wj * NJ * KK * 1024 + vo;
 #pragma unroll
-    for (int x = 0; x < NB * KK; ++x) {
-      const int op = (wi * NB * KK + x) * 1024 + vo, oq = (wj * NB * KK + x) * 1024 + vo;
-      f.ph[x] = *(const half8*)(buf + op);
-      f.qh[x] = *(const half8*)(buf + 8192 + oq);
-      f.ql[x] = *(const half8*)(buf + 12288 + oq);
-      f.pl[x] = *(const half8*)(buf + 4096 + op);
-    }
+    for (int x = 0; x < NI * KK; ++x) f.ph[x] = *(const half8*)(p + x * 1024);
+#pragma unroll
+    for (int x = 0; x < NJ * KK; ++x) f.qh[x] = *(const half8*)(q + x * 1024);
+#pragma unroll
+    for (int x = 0; x < NJ * KK; ++x) f.ql[x] = *(const half8*)(q + kQ + x * 1024);
+#pragma unroll
+    for (int x = 0; x < NI * KK; ++x) f.pl[x] = *(const half8*)(p + kP + x * 1024);
   };
 #define NS_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_f16(A, B, C, 0, 0, 0)
   auto multiply = [&](const Frag& f) {
-    if constexpr (NB == 1) {
+    if constexpr (NI == 1) {
       acc[0][0] = NS_MFMA(f.ph[0], f.qh[0], acc[0][0]);
       cr = NS_MFMA(f.ph[0], f.ql[0], cr);
       acc[0][0] = NS_MFMA(f.pl[0], f.qh[0], acc[0][0]);
@@ -275,17 +290,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       cr = NS_MFMA(f.pl[1], f.qh[1], cr);
     } else {
 #pragma unroll
-      for (int x = 0; x < NB; ++x)
+      for (int x = 0; x < NI; ++x)
 #pragma unroll
-        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.qh[y], acc[x][y]);
+        for (int y = 0; y < NJ; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.qh[y], acc[x][y]);
 #pragma unroll
-      for (int x = 0; x < NB; ++x)
+      for (int x = 0; x < NI; ++x)
 #pragma unroll
-        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.ql[y], acc[x][y]);
+        for (int y = 0; y < NJ; ++y) acc[x][y] = NS_MFMA(f.ph[x], f.ql[y], acc[x][y]);
 #pragma unroll
-      for (int x = 0; x < NB; ++x)
+      for (int x = 0; x < NI; ++x)
 #pragma unroll
-        for (int y = 0; y < NB; ++y) acc[x][y] = NS_MFMA(f.pl[x], f.qh[y], acc[x][y]);
+        for (int y = 0; y < NJ; ++y) acc[x][y] = NS_MFMA(f.pl[x], f.qh[y], acc[x][y]);
     }
   };
   // Step s multiplies stage s, whose fragments are in `cur`, and reads those of
@@ -329,17 +344,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       if (left > i) step(ks + i, NS_BUF(i), NS_BUF(i + 1), f[i & 1], f[(i + 1) & 1], left > i + 1, left > R + i);
   }
 #undef NS_BUF
-  if constexpr (NB == 1) acc[0][0] += cr;
+  if constexpr (NI == 1) acc[0][0] += cr;
   __syncthreads();
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
   unsigned* tr = (unsigned*)(w == 0 ? l0 : w == 1 ? l1 : w == 2 ? l2 : l3);
   const float lr = MODE == kFinal && a.momentum.p ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
 #pragma unroll
-  for (int x = 0; x < NB; ++x)
+  for (int x = 0; x < NI; ++x)
 #pragma unroll
-    for (int y = 0; y < NB; ++y) {
-      const int rbi = ti * TB + wi * NB + x, rbj = tj * TB + wj * NB + y;
+    for (int y = 0; y < NJ; ++y) {
+      const int rbi = ti * TI + wi * NI + x, rbj = tj * TJ + wj * NJ + y;
       if (rbi >= nPb || rbj >= nQb) continue;
+      // (128 x 64: a block above the diagonal belongs to the tile that holds its mirror)
+      if (NI != NJ && !rest && rbj / 2 > rbi / 2) continue;
       float v[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = acc[x][y][e] * g.f;
@@ -392,7 +409,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
           *(half4*)(Y + q * 512) = hv;
           *(half4*)(Y + g.y_lo + q * 512) = lv;
         }
-        if (MODE == kUpdate || ti != tj) {  // the other form: (row i, contraction j)
+        if (MODE == kUpdate || rbi / TJ != rbj / TJ) {  // the other form: (row i, contraction j)
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int e = 0; e < 16; ++e) tr[(8 * (e >> 2) + 4 * h + (e & 3)) * 33 + l31] = word[e];
@@ -768,18 +785,22 @@ int path_of(int64_t rows, int64_t cols) {
   return m <= 128 ? kThin128 : kTiled;
 }
 
-// Tiles of 128 or 64.  A launch lasts as long as its fullest CU: that many tiles,
-// a tile of 64 a quarter of one of 128 times 1.3 (its operands are read from LDS
-// for half as many products).  Measured, 128 / 64: six 1088 Gram matrices (270
-// tiles of 128) 41 / 33 us, their update (486) 54 / 62; one 1088 Gram (45) 23 / 11,
-// its update (81) 26 / 16; 2000 Gram (136) 44 / 42, its update (256) 54 / 76.
+// Tiles of 128 x 128, 128 x 64 (symmetric products) or 64 x 64.  A launch lasts as
+// long as its fullest CU; smaller tiles spread more evenly and read more of their
+// operands from LDS for a product.  Measured with 128 x 128 / 128 x 64 / 64 x 64:
+// six 1088 Gram matrices (270 / 486 / 918 tiles) 42 / 32 / 35 us, one (45 / 81 /
+// 153) 24 / 16 / 11; five steps of 2048 x 8192 (136 / 272 / 528) 2063 / 1994 /
+// 2131 us, of 4352 x 4352 (595 / 1190 / 2346) 4812 / 4791 / 6145, of twelve 1000 x
+// 1000 (432 / 864 / 1632) 939 / 980 / 1020 (4352 on another card: 4750 / 4965).  The update X <- B X, 128 x 128 / 64 x
+// 64: six 1088 (486 / 1734) 54 / 62 us, one (81 / 289) 26 / 16, one 2000 54 / 76.
 template <int MODE, int T>
 void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
+  constexpr bool kSym = MODE == kGram || MODE == kSquare;
   auto tiles = [&](int side) {  // whole tiles, and one more a side where a partial one follows
     const int tm = g.Rp / side, tn = g.Rq / side, pm = g.Rp % side != 0, pn = g.Rq % side != 0;
     g.ti = tm;
     g.tj = tn;
-    if (MODE == kGram || MODE == kSquare) {
+    if (kSym) {
       g.whole = tm * (tm + 1) / 2;
       g.rest = pm * (tm + 1);
     } else {
@@ -788,12 +809,29 @@ void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
     }
     return (g.whole + g.rest) * a.batch;
   };
+  auto pairs = [&]() {
+    const int c = (g.Rp + 63) / 64;
+    g.ti = c / 2;
+    g.whole = g.ti * (g.ti + 1);
+    g.rest = c % 2 * (g.ti + 1);
+    return (g.whole + g.rest) * a.batch;
+  };
+  auto rounds = [](int64_t n) { return (n + 255) / 256; };
+  if constexpr (kSym) {
+    if (tiles(64) > 384) {
+      const int64_t n = tiles(128), np = pairs();
+      if (13 * rounds(np) <= (n <= 256 ? 27 : 21 * rounds(n))) {
+        hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 2, 1>), dim3((unsigned)np), dim3(256), 0, s, g, a, p);
+        return;
+      }
+    }
+  }
   const int64_t n64 = tiles(64), n = tiles(128);
-  if (13 * ((n64 + 255) / 256) < 40 * ((n + 255) / 256)) {
+  if (kSym ? n64 <= 384 : 13 * rounds(n64) < 40 * rounds(n)) {
     tiles(64);
-    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 1>), dim3((unsigned)n64), dim3(256), 0, s, g, a, p);
+    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 1, 1>), dim3((unsigned)n64), dim3(256), 0, s, g, a, p);
   } else {
-    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 2>), dim3((unsigned)n), dim3(256), 0, s, g, a, p);
+    hipLaunchKernelGGL((ns_prod_kernel<MODE, T, 2, 2>), dim3((unsigned)n), dim3(256), 0, s, g, a, p);
   }
 }
 
