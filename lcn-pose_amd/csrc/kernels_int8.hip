@@ -27,20 +27,6 @@ __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 
 constexpr int64_t kPanelTokens = 1024;
 constexpr int64_t kGroupTokens = 16384;  // one workgroup of 64 a CU
 
-// 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
-template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
-template <int T>
-__device__ __forceinline__ void unpack_vec(v4u u, float (&v)[kVec<T>]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (T == kOpF32) v[i] = __uint_as_float(u[i]);
-    else if constexpr (T == kOpBF16) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
-    else {
-      v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)u[i]);
-      v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
-    }
-  }
-}
 // (kOnce: not kept in the caches, which then hold the integers for the product)
 template <int T, bool kOnce>
 __device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {

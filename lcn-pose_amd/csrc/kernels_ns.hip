@@ -32,6 +32,7 @@
 // 8-byte piece of the (row j, contraction i) form, and the other form is
 // transposed through LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "ops_common.h"
 
@@ -75,34 +76,57 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
 
 // ---- norm (and, for muon, the momentum update) ---------------------------------------------
 // part[b][p] = sum of squares, in float64, of the rows this workgroup walks.  A
-// wave takes a row at a time, 64 x kU elements in flight; bound by the read of
-// G (six 1088 x 1088: 28 us with one element in flight and 64 workgroups).
-constexpr int kU = 8;
-template <int T, bool kMuon>
+// wave takes a row at a time, kU pieces of kE elements a lane in flight (16 bytes
+// each where the rows are aligned, else single elements); bound by the read of G
+// (six 1088 x 1088: 28 us with one element in flight and 64 workgroups, 13.5 with
+// eight elements, 7.7 with five pieces; 4352 x 4352 bf16 58 and 15).
+template <int T, bool kMuon, bool kWide>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsArgs a, double* __restrict__ part) {
+  constexpr int kE = !kWide ? 1 : T == kOpF32 ? 4 : 8, kU = !kWide ? 8 : kMuon && T != kOpF32 ? 2 : 5;
   __shared__ double red[4];
   const int64_t b = blockIdx.y;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int pieces = a.cols / kE;
   double s = 0.0;
   for (int r = blockIdx.x * 4 + ty; r < a.rows; r += gridDim.x * 4) {
     const int64_t g0 = b * a.in.batch + (int64_t)r * a.in.row;
     float* mom = kMuon ? (float*)a.momentum.p + b * a.momentum.batch + (int64_t)r * a.momentum.row : nullptr;
-    for (int c0 = tx; c0 < a.cols; c0 += 64 * kU) {
-      float v[kU], m[kU];
+    for (int c0 = tx; c0 < pieces; c0 += 64 * kU) {
+      float v[kU][kE], m[kU][kE];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         const int c = c0 + 64 * u;
-        v[u] = c < a.cols ? op_load<T>(a.in.p, g0 + c) : 0.f;
-        if constexpr (kMuon) m[u] = c < a.cols ? mom[c] : 0.f;
+        const bool in = c < pieces;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) v[u][e] = m[u][e] = 0.f;
+        if constexpr (!kWide) {
+          if (in) v[u][0] = op_load<T>(a.in.p, g0 + c);
+          if (kMuon && in) m[u][0] = mom[c];
+        } else {
+          if (in) unpack_vec<T>(*(const v4u*)((const char*)a.in.p + (g0 + (int64_t)c * kE) * (16 / kE)), v[u]);
+          if constexpr (kMuon) {
+#pragma unroll
+            for (int e = 0; e < kE; e += 4)
+              if (in) unpack_vec<kOpF32>(*(const v4u*)(mom + c * kE + e), *(float(*)[4])(m[u] + e));
+          }
+        }
       }
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         if constexpr (kMuon) {
-          m[u] = fmaf(a.beta, m[u], v[u]);
-          if (c0 + 64 * u < a.cols) mom[c0 + 64 * u] = m[u];
-          v[u] = a.nesterov ? fmaf(a.beta, m[u], v[u]) : m[u];
+#pragma unroll
+          for (int e = 0; e < kE; ++e) m[u][e] = fmaf(a.beta, m[u][e], v[u][e]);
+          if (c0 + 64 * u < pieces) {
+            if constexpr (!kWide) mom[c0 + 64 * u] = m[u][0];
+            else
+#pragma unroll
+              for (int e = 0; e < kE; e += 4) *(float4*)(mom + (c0 + 64 * u) * kE + e) = make_float4(m[u][e], m[u][e + 1], m[u][e + 2], m[u][e + 3]);
+          }
+#pragma unroll
+          for (int e = 0; e < kE; ++e) v[u][e] = a.nesterov ? fmaf(a.beta, m[u][e], v[u][e]) : m[u][e];
         }
-        s = fma((double)v[u], (double)v[u], s);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) s = fma((double)v[u][e], (double)v[u][e], s);
       }
     }
   }
@@ -123,53 +147,92 @@ __device__ __forceinline__ double norm2_of(const double* __restrict__ part, int 
 }
 
 // ---- X0 in both orientations ---------------------------------------------------------------
+// A workgroup takes 32 rows x 32 kInit columns of X, all its loads in flight
+// together; bound by memory (G once, four planes written: six 1088 x 1088 in 21 us,
+// 28 with one block of columns a workgroup).
+constexpr int kInit = 4;
 template <int T, bool kMuon>
 __global__ __launch_bounds__(256) void ns_init_kernel(NsArgs a, NsPlan p, int parts, const double* __restrict__ part,
                                                       char* __restrict__ ws) {
-  __shared__ unsigned tile[32 * 33];
+  __shared__ unsigned tile[kInit][32 * 33];
   const int64_t b = blockIdx.y;
-  const int nb = p.np / 32;
-  const int bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;  // 32-row block of X, 32-column block
+  const int nb = p.np / 32, strips = (nb + kInit - 1) / kInit;
+  const int bi = blockIdx.x / strips, bj0 = (blockIdx.x - bi * strips) * kInit;  // 32-row block of X, first 32-column block
+  const bool tall = a.rows > a.cols;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  float v[kInit][4], m[kInit][4];
+#pragma unroll
+  for (int z = 0; z < kInit; ++z)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // fast index tx along the source's rows; (i, j) of X
+      const int sr = ty + 8 * q;
+      const int gi = bi * 32 + (tall ? tx : sr), gj = (bj0 + z) * 32 + (tall ? sr : tx);
+      const bool in = gi < p.m && gj < p.n;
+      const int64_t r = tall ? gj : gi, c = tall ? gi : gj;
+      v[z][q] = in ? op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c) : 0.f;
+      if constexpr (kMuon) m[z][q] = in ? ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c] : 0.f;
+    }
   const double s = norm2_of(part + b * kNormParts, parts);
   const double inv = (double)kSx / fmax(sqrt(s), (double)a.eps);
   const bool bad = !(s < 1e300);  // an infinity or a NaN in the matrix: every entry becomes NaN
-  const bool tall = a.rows > a.cols;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    // fast index tx along the source's rows; (i, j) of X
-    const int sr = ty + 8 * q;
-    const int i = tall ? tx : sr, j = tall ? sr : tx;
-    const int gi = bi * 32 + i, gj = bj * 32 + j;
-    float v = 0.f;
-    if (gi < p.m && gj < p.n) {
-      const int64_t r = tall ? gj : gi, c = tall ? gi : gj;
-      v = op_load<T>(a.in.p, b * a.in.batch + r * a.in.row + c);
-      if constexpr (kMuon) {
-        const float m = ((const float*)a.momentum.p)[b * a.momentum.batch + r * a.momentum.row + c];
-        v = a.nesterov ? fmaf(a.beta, m, v) : m;
-      }
-      v = bad ? __builtin_nanf("") : (float)((double)v * inv);
+  for (int z = 0; z < kInit; ++z)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int sr = ty + 8 * q, i = tall ? tx : sr, j = tall ? sr : tx;
+      const int gi = bi * 32 + i, gj = (bj0 + z) * 32 + j;
+      float u = v[z][q];
+      if constexpr (kMuon) u = a.nesterov ? fmaf(a.beta, m[z][q], u) : m[z][q];
+      u = gi < p.m && gj < p.n ? bad ? __builtin_nanf("") : (float)((double)u * inv) : 0.f;
+      _Float16 hi, lo;
+      split(u, hi, lo);
+      tile[z][i * 33 + j] = (unsigned)__builtin_bit_cast(unsigned short, hi) | ((unsigned)__builtin_bit_cast(unsigned short, lo) << 16);
     }
-    _Float16 hi, lo;
-    split(v, hi, lo);
-    tile[i * 33 + j] = (unsigned)__builtin_bit_cast(unsigned short, hi) | ((unsigned)__builtin_bit_cast(unsigned short, lo) << 16);
-  }
   __syncthreads();
   // 32 x 4 octets in either form: threads 0..127 Xr (row i, contraction j), 128..255 Xc
   const int t = threadIdx.x & 127, row = t & 31, u = t >> 5;
   const bool xc = threadIdx.x >= 128;
-  unsigned short hs[8], ls[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const unsigned w = xc ? tile[(8 * u + e) * 33 + row] : tile[row * 33 + 8 * u + e];
-    hs[e] = (unsigned short)w;
-    ls[e] = (unsigned short)(w >> 16);
+  for (int z = 0; z < kInit; ++z) {
+    const int bj = bj0 + z;
+    if (bj >= nb) break;
+    unsigned short hs[8], ls[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned w = xc ? tile[z][(8 * u + e) * 33 + row] : tile[z][row * 33 + 8 * u + e];
+      hs[e] = (unsigned short)w;
+      ls[e] = (unsigned short)(w >> 16);
+    }
+    const int64_t unit = xc ? ((int64_t)bj * (p.mp / 8) + bi * 4 + u) * 32 + row : ((int64_t)bi * (p.np / 8) + bj * 4 + u) * 32 + row;
+    char* x = ws + b * p.stride + p.x[0] + (xc ? 2 * p.xplane : 0);
+    *(v4u*)(x + unit * 16) = *(v4u*)hs;
+    *(v4u*)(x + p.xplane + unit * 16) = *(v4u*)ls;
   }
-  const int64_t unit = xc ? ((int64_t)bj * (p.mp / 8) + bi * 4 + u) * 32 + row : ((int64_t)bi * (p.np / 8) + bj * 4 + u) * 32 + row;
-  char* x = ws + b * p.stride + p.x[0] + (xc ? 2 * p.xplane : 0);
-  *(v4u*)(x + unit * 16) = *(v4u*)hs;
-  *(v4u*)(x + p.xplane + unit * 16) = *(v4u*)ls;
+}
+
+// one element or four aligned neighbours of a row
+template <int E>
+__device__ __forceinline__ void load_some(const float* p, int64_t o, float (&v)[E]) {
+  if constexpr (E == 1) {
+    v[0] = p[o];
+  } else {
+    const float4 f = *(const float4*)(p + o);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  }
+}
+template <int T, int E>
+__device__ __forceinline__ void store_some(void* p, int64_t o, const float (&v)[E]) {
+  if constexpr (E == 1) {
+    op_store<T>(p, o, v[0]);
+  } else if constexpr (T == kOpF32) {
+    *(float4*)((float*)p + o) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    half4 u;  // four 16-bit values of either type
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = T == kOpF16 ? (_Float16)v[e] : __builtin_bit_cast(_Float16, (__bf16)v[e]);
+    *(half4*)((_Float16*)p + o) = u;
+  }
 }
 
 // ---- the three products --------------------------------------------------------------------
@@ -349,6 +412,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
   unsigned* tr = (unsigned*)(w == 0 ? l0 : w == 1 ? l1 : w == 2 ? l2 : l3);
   const float lr = MODE == kFinal && a.momentum.p ? (a.lr_dev ? *a.lr_dev : a.lr) : 0.f;
+  const int out_bytes = a.momentum.p || T == kOpF32 ? 16 : 8;  // of four neighbours
+  const bool wide = MODE == kFinal && ((uintptr_t)a.out.p % out_bytes | a.cols % 4 | a.out.row % 4 | (a.batch > 1 ? a.out.batch % 4 : 0)) == 0;
 #pragma unroll
   for (int x = 0; x < NI; ++x)
 #pragma unroll
@@ -375,23 +440,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
           for (int e = 0; e < 16; ++e) v[e] += 8 * (e >> 2) + 4 * h + (e & 3) == l31 ? a.a * kSb : 0.f;
       }
       if constexpr (MODE == kFinal) {
+        // through LDS, so that a wave's lanes follow the output's rows: four elements
+        // a lane where they are aligned, else one (parameters: all loads before the
+        // first store)
         const bool tall = a.rows > a.cols;
-        const int j = rbj * 32 + l31;
-        if (j >= pl.n) continue;
-        int64_t o[16];
-        float W[16];
+        float* block = (float*)tr;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int i = rbi * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-          o[e] = i < pl.m ? (int64_t)mat * a.out.batch + (int64_t)(tall ? j : i) * a.out.row + (tall ? i : j) : -1;
-          if (a.momentum.p) W[e] = o[e] >= 0 ? ((const float*)a.out.p)[o[e]] : 0.f;  // all in flight before the first store
+          const int i = 8 * (e >> 2) + 4 * h + (e & 3);
+          block[tall ? l31 * 33 + i : i * 33 + l31] = v[e];
         }
+        __builtin_amdgcn_wave_barrier();
+        auto write = [&](auto four) {
+          constexpr int E = decltype(four)::value ? 4 : 1, kQ = 16 / E, kRow = 32 / E;  // pieces of E, kRow lanes a row
+          const int lr0 = lane / kRow, lc = lane % kRow * E;
+          const int r0 = 32 * (tall ? rbj : rbi) + lr0, c0 = 32 * (tall ? rbi : rbj) + lc;  // of the output
+          if (c0 >= a.cols) return;
+          float D[kQ][E], W[kQ][E];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (o[e] < 0) continue;
-          if (a.momentum.p) ((float*)a.out.p)[o[e]] = fmaf(-lr * a.scale, v[e], W[e] * (1.f - lr * a.decay));
-          else op_store<T>(a.out.p, o[e], v[e]);
-        }
+          for (int q = 0; q < kQ; ++q) {
+            const int r = r0 + 64 / kRow * q;
+            if (a.momentum.p && r < a.rows) load_some((const float*)a.out.p, (int64_t)mat * a.out.batch + (int64_t)r * a.out.row + c0, W[q]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) D[q][e] = block[(lr0 + 64 / kRow * q) * 33 + lc + e];
+          }
+#pragma unroll
+          for (int q = 0; q < kQ; ++q) {
+            const int r = r0 + 64 / kRow * q;
+            if (r >= a.rows) continue;
+            const int64_t o = (int64_t)mat * a.out.batch + (int64_t)r * a.out.row + c0;
+            if (a.momentum.p) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) D[q][e] = fmaf(-lr * a.scale, D[q][e], W[q][e] * (1.f - lr * a.decay));
+              store_some<kOpF32>(a.out.p, o, D[q]);
+            } else {
+              store_some<T>(a.out.p, o, D[q]);
+            }
+          }
+        };
+        if (wide) write(std::true_type{});
+        else write(std::false_type{});
+        __builtin_amdgcn_wave_barrier();
       } else {
         char* Y = g.Y + mat * g.stride + at;
         unsigned word[16];
@@ -745,7 +835,12 @@ __global__ __launch_bounds__(64 * NW) void ns_thin_kernel(NsArgs a, ThinPlan p, 
 
 template <int T, bool kMuon>
 void launch_norm(const NsArgs& a, int parts, double* part, hipStream_t s) {
-  hipLaunchKernelGGL((ns_norm_kernel<T, kMuon>), dim3(parts, (unsigned)a.batch), dim3(256), 0, s, a, part);
+  constexpr int kE = T == kOpF32 ? 4 : 8;
+  bool wide = ((uintptr_t)a.in.p % 16 | a.cols % kE | a.in.row % kE | (a.batch > 1 ? a.in.batch % kE : 0)) == 0;
+  if (kMuon) wide = wide && ((uintptr_t)a.momentum.p % 16 | a.momentum.row % 4 | (a.batch > 1 ? a.momentum.batch % 4 : 0)) == 0;
+  const dim3 grid(parts, (unsigned)a.batch);
+  if (wide) hipLaunchKernelGGL((ns_norm_kernel<T, kMuon, true>), grid, dim3(256), 0, s, a, part);
+  else hipLaunchKernelGGL((ns_norm_kernel<T, kMuon, false>), grid, dim3(256), 0, s, a, part);
 }
 // workgroups of the norm for a matrix: four rows at a time each, ~1 000 in all
 int norm_parts(const NsArgs& a) {
@@ -791,8 +886,9 @@ int path_of(int64_t rows, int64_t cols) {
 // six 1088 Gram matrices (270 / 486 / 918 tiles) 42 / 32 / 35 us, one (45 / 81 /
 // 153) 24 / 16 / 11; five steps of 2048 x 8192 (136 / 272 / 528) 2063 / 1994 /
 // 2131 us, of 4352 x 4352 (595 / 1190 / 2346) 4812 / 4791 / 6145, of twelve 1000 x
-// 1000 (432 / 864 / 1632) 939 / 980 / 1020 (4352 on another card: 4750 / 4965).  The update X <- B X, 128 x 128 / 64 x
-// 64: six 1088 (486 / 1734) 54 / 62 us, one (81 / 289) 26 / 16, one 2000 54 / 76.
+// 1000 (432 / 864 / 1632) 939 / 980 / 1020 (4352 on another card 4750 / 4965).  The
+// update X <- B X, 128 x 128 / 64 x 64: six 1088 (486 / 1734) 54 / 62 us, one (81 /
+// 289) 26 / 16, one 2000 54 / 76.
 template <int MODE, int T>
 void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
   constexpr bool kSym = MODE == kGram || MODE == kSquare;
@@ -847,7 +943,7 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
   const int parts = norm_parts(a);
   launch_norm<T, kMuon>(a, parts, part, s);
-  hipLaunchKernelGGL((ns_init_kernel<T, kMuon>), dim3((p.mp / 32) * (p.np / 32), (unsigned)a.batch), dim3(256), 0, s, a, p, parts, part, ws);
+  hipLaunchKernelGGL((ns_init_kernel<T, kMuon>), dim3((p.mp / 32) * ((p.np / 32 + kInit - 1) / kInit), (unsigned)a.batch), dim3(256), 0, s, a, p, parts, part, ws);
   int cur = 0;
   for (int k = 0; k < a.steps; ++k, cur ^= 1) {
     char *xr = ws + p.x[cur], *xc = xr + 2 * p.xplane, *yr = ws + p.x[cur ^ 1], *yc = yr + 2 * p.xplane;

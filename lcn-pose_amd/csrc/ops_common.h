@@ -25,6 +25,21 @@ __device__ __forceinline__ void op_store(void* p, int64_t e, float v) {
   else ((_Float16*)p)[e] = (_Float16)v;
 }
 
+// 16 bytes of a row as floats: 4 of fp32, 8 of the 16-bit types
+template <int T> constexpr int kVec = T == kOpF32 ? 4 : 8;
+template <int T>
+__device__ __forceinline__ void unpack_vec(v4u u, float (&v)[kVec<T>]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == kOpF32) v[i] = __uint_as_float(u[i]);
+    else if constexpr (T == kOpBF16) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    else {
+      v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)u[i]);
+      v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
+    }
+  }
+}
+
 // ---- int8 quantisation of a row --------------------------------------------------------------
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100: a row below it counts as zero
 
