@@ -27,12 +27,6 @@ __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 
 constexpr int64_t kPanelTokens = 1024;
 constexpr int64_t kGroupTokens = 16384;  // one workgroup of 64 a CU
 
-// (kOnce: not kept in the caches, which then hold the integers for the product)
-template <int T, bool kOnce>
-__device__ __forceinline__ void load_vec(const void* p, int64_t e, float (&v)[kVec<T>]) {
-  const v4u* at = (const v4u*)((const char*)p + e * (16 / kVec<T>));
-  unpack_vec<T>(kOnce ? __builtin_nontemporal_load(at) : *at, v);
-}
 // largest magnitude of a wave's values, and whether one is an infinity or a NaN
 __device__ __forceinline__ void wave_top(float& top, bool& bad) {
 #pragma unroll
@@ -45,99 +39,116 @@ __device__ __forceinline__ void see(float v, float& top, bool& bad) {
   top = fmaxf(top, v);
 }
 
+// Rows are read 16 bytes at a time at any alignment; what a row has past its last
+// whole piece comes an element a lane (`tail_piece`).  kOnce: not kept in the
+// caches, which then hold the integers for the product.
+typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned u32_any __attribute__((aligned(1)));
+template <int T> constexpr int kElem = 16 / kVec<T>;  // bytes
+template <int T>
+__device__ __forceinline__ v4u tail_piece(const void* p, int64_t e, int rem, int lane) {
+  unsigned b = 0;
+  if (lane < rem) b = T == kOpF32 ? ((const unsigned*)p)[e + lane] : ((const unsigned short*)p)[e + lane];
+  v4u u;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) u[d] = T == kOpF32 ? __shfl(b, d) : __shfl(b, 2 * d) | __shfl(b, 2 * d + 1) << 16;
+  return u;
+}
+// piece c of the row at element r: one of the `whole` pieces, the tail, or zeros
+template <int T, bool kOnce>
+__device__ __forceinline__ v4u row_piece(const void* p, int64_t r, int c, int whole, v4u tail) {
+  v4u u = {0, 0, 0, 0};
+  if (c < whole) {
+    const v4u_any* at = (const v4u_any*)((const char*)p + (r + (int64_t)c * kVec<T>) * kElem<T>);
+    u = kOnce ? __builtin_nontemporal_load(at) : *at;
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d) u[d] = c == whole ? tail[d] : u[d];
+  return u;
+}
+template <int T>
+__device__ __forceinline__ void see_piece(v4u u, float& top, bool& bad) {
+  float v[kVec<T>];
+  unpack_vec<T>(u, v);
+#pragma unroll
+  for (int e = 0; e < kVec<T>; ++e) see(v[e], top, bad);
+}
+// the piece's integers, kVec bytes at `o`
+template <int T>
+__device__ __forceinline__ void put_piece(void* o, v4u u, float factor, bool bad) {
+  float v[kVec<T>];
+  unpack_vec<T>(u, v);
+  if constexpr (kVec<T> == 4) *(unsigned*)o = quant4(v[0], v[1], v[2], v[3], factor, bad);
+  else *(uint2*)o = make_uint2(quant4(v[0], v[1], v[2], v[3], factor, bad), quant4(v[4], v[5], v[6], v[7], factor, bad));
+}
+// 16 weights from p (at + 16 may pass the row: zeros of the tokens meet what is
+// there; at the end of the weights, byte by byte)
+__device__ __forceinline__ v4i weights16(const int8_t* p, int left, const int8_t* end) {
+  v4i v = {0, 0, 0, 0};
+  if (p + 16 <= end) {
+    v = *(const v4i_any*)p;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (e < left) v[e >> 2] |= (int)((unsigned)(uint8_t)p[e] << (8 * (e & 3)));
+  }
+  return v;
+}
 // One wave a row: largest magnitude, then the integers, rows padded to kp with
-// zeros.  kPieces > 0: rows of whole 16-byte pieces, of which a lane keeps up to
-// kPieces in registers between the two passes; what is past them is read again
-// (from L2).  kPieces = 0: any alignment, an element at a time.  Bound by memory:
-// 65 536 x 1088 fp32 in 60 us (5.9 TB/s).  x is read past the caches: with it in
-// them, the integers had to come from memory again (77 us here, and 140 instead
-// of 98 us in the product).
-template <int T, int kPieces>
+// zeros.  A lane keeps up to kRegs pieces in registers between the two passes; what
+// is past them is read again (from L2).  Bound by memory: 65 536 x 1088 fp32 in 60 us
+// (5.9 TB/s).  x is read past the caches: with it in them, the integers had to come
+// from memory again (77 us here, and 140 instead of 98 us in the product).
+template <int T, int kRegs>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict__ x, int64_t x_row, int64_t tokens, int k,
                                                          int64_t kp, int8_t* __restrict__ q, float* __restrict__ scale) {
+  constexpr int V = kVec<T>;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (t >= tokens) return;
   float top = 0.f, factor, s;
   bool bad = false;
-  const int64_t r = t * x_row;
+  const int64_t r = t * x_row, panel = tokens * 64;
   int8_t* out = q + t * 64;
-  const int64_t panel = tokens * 64;
-  if constexpr (kPieces > 0) {
-    constexpr int V = kVec<T>, kRegs = kPieces;
-    const int pieces = k / V;  // k is a multiple of V here
-    float keep[kRegs][V];
+  const int whole = k / V, padded = (int)(kp / V);
+  v4u keep[kRegs], tail = {0, 0, 0, 0};
+  if (k % V) tail = tail_piece<T>(x, r + (int64_t)whole * V, k % V, lane);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      if (lane + 64 * i < pieces) load_vec<T, true>(x, r + (int64_t)(lane + 64 * i) * V, keep[i]);
-      else
+  for (int i = 0; i < kRegs; ++i) keep[i] = row_piece<T, true>(x, r, lane + 64 * i, whole, tail);
 #pragma unroll
-        for (int e = 0; e < V; ++e) keep[i][e] = 0.f;
-    }
+  for (int i = 0; i < kRegs; ++i) see_piece<T>(keep[i], top, bad);
+  for (int c = lane + 64 * kRegs; c <= whole; c += 64) see_piece<T>(row_piece<T, false>(x, r, c, whole, tail), top, bad);
+  wave_top(top, bad);
+  row_scale(top, bad, factor, s);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) see(keep[i][e], top, bad);
-    for (int c = lane + 64 * kRegs; c < pieces; c += 64) {
-      float v[V];
-      load_vec<T, false>(x, r + (int64_t)c * V, v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) see(v[e], top, bad);
-    }
-    wave_top(top, bad);
-    row_scale(top, bad, factor, s);
-    auto put = [&](int c, const float (&v)[V]) {
-      unsigned w[V / 4];
-#pragma unroll
-      for (int d = 0; d < V / 4; ++d) w[d] = quant4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3], factor, bad);
-      int8_t* o = out + (c * V >> 6) * panel + (c * V & 63);
-      if constexpr (V == 4) *(unsigned*)o = w[0];
-      else *(uint2*)o = make_uint2(w[0], w[1]);
-    };
-    const int padded = (int)(kp / V);  // the pieces past k hold zeros
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (lane + 64 * i < padded) put(lane + 64 * i, keep[i]);
-    for (int c = lane + 64 * kRegs; c < padded; c += 64) {
-      float v[V] = {};
-      if (c < pieces) load_vec<T, false>(x, r + (int64_t)c * V, v);
-      put(c, v);
-    }
-  } else {
-    constexpr int kRegs = 16;
-    float keep[kRegs];
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) keep[i] = lane + 64 * i < k ? op_load<T>(x, r + lane + 64 * i) : 0.f;
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) see(keep[i], top, bad);
-    for (int c = lane + 64 * kRegs; c < k; c += 64) see(op_load<T>(x, r + c), top, bad);
-    wave_top(top, bad);
-    row_scale(top, bad, factor, s);
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (64 * i < kp) out[i * panel + lane] = bad ? (int8_t)0 : quant(keep[i], factor);
-    for (int c = lane + 64 * kRegs; c < kp; c += 64) out[(c >> 6) * panel + lane] = c < k && !bad ? quant(op_load<T>(x, r + c), factor) : (int8_t)0;
+  for (int i = 0; i < kRegs; ++i) {
+    const int c = lane + 64 * i;
+    if (c < padded) put_piece<T>(out + (c * V >> 6) * panel + (c * V & 63), keep[i], factor, bad);
   }
+  for (int c = lane + 64 * kRegs; c < padded; c += 64)
+    put_piece<T>(out + (c * V >> 6) * panel + (c * V & 63), row_piece<T, false>(x, r, c, whole, tail), factor, bad);
   if (lane == 0) scale[t] = s;
 }
 
-// weight rows of any alignment -> panels of 64 of K, zero padded; kAligned: rows of
-// whole 4-byte pieces
-template <bool kAligned>
-__global__ __launch_bounds__(256) void panels_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int8_t* __restrict__ out) {
-  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // channel
-  if (c >= n) return;
-  const int k0 = blockIdx.y * 64 + (threadIdx.x & 15) * 4;
-  const int8_t* src = w + c * w_row + k0;
+// four weights of a row from k0 on, zeros past K
+__device__ __forceinline__ unsigned weights4(const int8_t* row, int k0, int k) {
   unsigned v = 0;
-  if constexpr (kAligned) {
-    if (k0 < k) v = *(const unsigned*)src;
+  if (k0 + 4 <= k) {
+    v = *(const u32_any*)(row + k0);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (k0 + e < k) v |= (unsigned)(uint8_t)src[e] << (8 * e);
+      if (k0 + e < k) v |= (unsigned)(uint8_t)row[k0 + e] << (8 * e);
   }
-  *(unsigned*)(out + ((int64_t)blockIdx.y * n + c) * 64 + (threadIdx.x & 15) * 4) = v;
+  return v;
+}
+// weight rows -> panels of 64 of K, zero padded
+__global__ __launch_bounds__(256) void panels_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int8_t* __restrict__ out) {
+  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // channel
+  if (c >= n) return;
+  const int at = (threadIdx.x & 15) * 4;
+  *(unsigned*)(out + ((int64_t)blockIdx.y * n + c) * 64 + at) = weights4(w + c * w_row, blockIdx.y * 64 + at, k);
 }
 
 #define I8_LDS(SRC, VOFF, SOFF, DST) \
@@ -326,11 +337,7 @@ constexpr int kGroupLds = 80 * 1024 - 512;   // half a CU's
 __global__ __launch_bounds__(256) void fragments_kernel(const int8_t* __restrict__ w, int64_t w_row, int n, int k, int kp, int8_t* __restrict__ out) {
   const int c = blockIdx.x * 16 + (threadIdx.x >> 4);  // channel, up to n rounded up to 64
   const int k0 = blockIdx.y * 64 + (threadIdx.x & 15) * 4;
-  const int8_t* src = w + (int64_t)c * w_row + k0;
-  unsigned v = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (c < n && k0 + e < k) v |= (unsigned)(uint8_t)src[e] << (8 * e);
+  const unsigned v = c < n ? weights4(w + (int64_t)c * w_row, k0, k) : 0u;
   *(unsigned*)(out + (int64_t)(c >> 5) * kp * 32 + (k0 >> 5) * 1024 + ((k0 >> 4) & 1) * 512 + (c & 31) * 16 + (k0 & 15)) = v;
 }
 
@@ -361,17 +368,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   {
     // four groups of four rows a wave, the next group's loads in flight
     constexpr int V = kVec<T>, kRegs = T == kOpF32 ? 5 : 3, kRows = 4;
-    const int pieces = k / V, padded = (int)(g.kp / V);
+    const int whole = k / V, padded = (int)(g.kp / V);
     struct Rows { v4u u[kRows][kRegs]; };
     auto load = [&](int r0, Rows& m) {
 #pragma unroll
-      for (int j = 0; j < kRows; ++j)
+      for (int j = 0; j < kRows; ++j) {
+        const int64_t r = (t0 + min(r0 + j, trows - 1)) * x_row;
+        v4u tail = {0, 0, 0, 0};
+        if (k % V) tail = tail_piece<T>(x, r + (int64_t)whole * V, k % V, lane);
 #pragma unroll
-        for (int i = 0; i < kRegs; ++i) {
-          m.u[j][i] = v4u{0, 0, 0, 0};
-          if (lane + 64 * i < pieces)
-            m.u[j][i] = __builtin_nontemporal_load((const v4u*)((const char*)x + (t0 + min(r0 + j, trows - 1)) * x_row * (16 / V) + (lane + 64 * i) * 16));
-        }
+        for (int i = 0; i < kRegs; ++i) m.u[j][i] = row_piece<T, true>(x, r, lane + 64 * i, whole, tail);
+      }
     };
     auto quantise = [&](int r0, const Rows& m) {
       float top[kRows];
@@ -381,12 +388,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         top[j] = 0.f;
         bad[j] = false;
 #pragma unroll
-        for (int i = 0; i < kRegs; ++i) {
-          float v[V];
-          unpack_vec<T>(m.u[j][i], v);
-#pragma unroll
-          for (int e = 0; e < V; ++e) see(v[e], top[j], bad[j]);
-        }
+        for (int i = 0; i < kRegs; ++i) see_piece<T>(m.u[j][i], top[j], bad[j]);
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j) wave_top(top[j], bad[j]);
@@ -399,13 +401,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
           const int at = (lane + 64 * i) * V, u = at >> 4;
-          if (lane + 64 * i < padded) {
-            float v[V];
-            unpack_vec<T>(m.u[j][i], v);
-            char* p = lds + (u >> 1) * 2048 + (r >> 5) * 1024 + (u & 1) * 512 + ((r ^ u) & 31) * 16 + (at & 15);
-            if constexpr (V == 4) *(unsigned*)p = quant4(v[0], v[1], v[2], v[3], factor, bad[j]);
-            else *(uint2*)p = make_uint2(quant4(v[0], v[1], v[2], v[3], factor, bad[j]), quant4(v[4], v[5], v[6], v[7], factor, bad[j]));
-          }
+          if (lane + 64 * i < padded)
+            put_piece<T>(lds + (u >> 1) * 2048 + (r >> 5) * 1024 + (u & 1) * 512 + ((r ^ u) & 31) * 16 + (at & 15), m.u[j][i], factor, bad[j]);
         }
       }
     };
@@ -536,7 +533,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 constexpr int kFewTokens = 16;
 constexpr int kFewLds = 65536;   // bytes of quantised tokens a workgroup holds
 
-template <int T, bool kFused, bool kAligned>
+template <int T, bool kFused>
 __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ int red[4][256];
@@ -547,18 +544,10 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
   const int n0 = blockIdx.x * 16;
   const int c16 = lane & 15, kq = lane >> 4;  // channel (or token) of the fragment, its 16-byte quarter of a piece
   const int8_t* wrow = g.w + (int64_t)min(n0 + c16, g.n - 1) * g.w_row;
+  const int8_t* wend = g.w + g.w_bytes;
   auto weights = [&](int ks) {
     const int at = ks * 64 + kq * 16;
-    v4i v = {0, 0, 0, 0};
-    if constexpr (kAligned) {
-      // a 16-byte piece may end past the row: it stays inside it where k is a multiple of 16
-      if (at < k) v = *(const v4i*)(wrow + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (at + e < k) v[e >> 2] |= (int)((unsigned)(uint8_t)wrow[at + e] << (8 * (e & 3)));
-    }
-    return v;
+    return at < k ? weights16(wrow + at, k - at, wend) : v4i{0, 0, 0, 0};
   };
   const int nk = kp / 64;
   constexpr int kAhead = 4;  // pieces of a wave in flight
@@ -628,6 +617,101 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
   }
 }
 
+// ---- up to some hundred tokens ---------------------------------------------------------------
+// A workgroup takes 16 tokens x 64 channels: it quantises the tokens into LDS, four
+// rows a wave with all their loads in flight, each of the n / 64 workgroups anew
+// (they come from L2), and a wave multiplies them by 16 channels, whose weights
+// are asked for before the quantisation starts.  One launch, no workspace.  Bound
+// by latency (the rows, their largest magnitude, the weights of the second half of
+// K): 200 x 1088 x 1088 in 7.5 us.
+constexpr int kMidAhead = 6;  // 64-byte pieces of K in flight
+template <int T>
+__global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float qs[16];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kp = (int)g.kp, nk = kp / 64, pitch = kp + 16;
+  const int64_t t0 = (int64_t)blockIdx.x * 16;
+  const int rows = (int)min((int64_t)16, g.tokens - t0);
+  const int c16 = lane & 15, kq = lane >> 4, n0 = blockIdx.y * 64 + w * 16;
+  // channels past the last repeat it, K past its end meets zeros of the tokens
+  const int8_t* wrow = g.w + (int64_t)min(n0 + c16, g.n - 1) * g.w_row;
+  const int8_t* wend = g.w + g.w_bytes;
+  auto weights = [&](int ks) {
+    const int at = ks * 64 + kq * 16;
+    return at < k ? weights16(wrow + at, k - at, wend) : v4i{0, 0, 0, 0};
+  };
+  v4i wv[kMidAhead];
+#pragma unroll
+  for (int i = 0; i < kMidAhead; ++i) wv[i] = weights(i);
+  {
+    // the first kRegs pieces of four rows stay in registers
+    constexpr int V = kVec<T>, kRegs = T == kOpF32 ? 5 : 3, kRows = 4;
+    const int whole = k / V, padded = kp / V;
+    int64_t r[kRows];
+    v4u keep[kRows][kRegs], tail[kRows];
+    float top[kRows];
+    bool bad[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      r[j] = (t0 + min(w * 4 + j, rows - 1)) * x_row;
+      tail[j] = v4u{0, 0, 0, 0};
+      if (k % V) tail[j] = tail_piece<T>(x, r[j] + (int64_t)whole * V, k % V, lane);
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) keep[j][i] = row_piece<T, false>(x, r[j], lane + 64 * i, whole, tail[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      top[j] = 0.f;
+      bad[j] = false;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) see_piece<T>(keep[j][i], top[j], bad[j]);
+    }
+    for (int c = lane + 64 * kRegs; c <= whole; c += 64)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) see_piece<T>(row_piece<T, false>(x, r[j], c, whole, tail[j]), top[j], bad[j]);
+    float factor[kRows];
+    char* o = lds + w * 4 * pitch;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      float s;
+      wave_top(top[j], bad[j]);
+      row_scale(top[j], bad[j], factor[j], s);
+      if (lane == 0) qs[w * 4 + j] = s;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i)
+        if (lane + 64 * i < padded) put_piece<T>(o + j * pitch + (lane + 64 * i) * V, keep[j][i], factor[j], bad[j]);
+    }
+    for (int c = lane + 64 * kRegs; c < padded; c += 64)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) put_piece<T>(o + j * pitch + c * V, row_piece<T, false>(x, r[j], c, whole, tail[j]), factor[j], bad[j]);
+  }
+  __syncthreads();
+  v4i acc = {0, 0, 0, 0};
+  const char* a = lds + c16 * pitch + kq * 16;
+  for (int ks = 0; ks < nk; ks += kMidAhead) {
+#pragma unroll
+    for (int i = 0; i < kMidAhead; ++i) {
+      if (ks + i >= nk) break;
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(a + (ks + i) * 64), wv[i], acc, 0, 0, 0);
+      wv[i] = weights(ks + i + kMidAhead);
+    }
+  }
+  // lane holds tokens 4 kq .. 4 kq + 3 of channel c16
+  const int n = n0 + c16;
+  if (n < g.n) {
+    const float sw = g.ws[n], b = g.bias ? g.bias[n] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = 4 * kq + e;
+      if (t >= rows) continue;
+      float v = (float)acc[e] * qs[t] * sw;
+      if (g.bias) v += b;
+      op_store<T>(g.out, (t0 + t) * g.out_row + n, v);
+    }
+  }
+}
+
 // one wave a channel: largest magnitude over k, then the integers
 template <int T>
 __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWArgs a) {
@@ -652,13 +736,10 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWArgs a) {
 
 template <int T>
 void launch_quant_rows(const Int8Args& a, int64_t kp, int8_t* q, float* qs, hipStream_t s) {
-  constexpr int V = kVec<T>;
-  const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && (a.x_row % V == 0 || a.tokens == 1);
   const dim3 grid((unsigned)((a.tokens + 3) / 4));
   constexpr int kMany = T == kOpF32 ? 18 : 9;  // K up to 4608 in registers
-  if (al && a.k <= 64 * 5 * V) hipLaunchKernelGGL((quant_rows_kernel<T, 5>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
-  else if (al) hipLaunchKernelGGL((quant_rows_kernel<T, kMany>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
-  else hipLaunchKernelGGL((quant_rows_kernel<T, 0>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  if (a.k <= 64 * 5 * kVec<T>) hipLaunchKernelGGL((quant_rows_kernel<T, 5>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
+  else hipLaunchKernelGGL((quant_rows_kernel<T, kMany>), grid, dim3(256), 0, s, a.x, a.x_row, a.tokens, a.k, kp, q, qs);
 }
 
 template <int T, int BI, int BJ, int R>
@@ -671,6 +752,15 @@ void launch_tiles(Int8Gemm& g, hipStream_t s) {
 // every workgroup quantises the tokens for itself while that is little work
 bool fused(int64_t tokens, int64_t k) {
   return tokens <= kFewTokens && tokens * (pad64(k) + 16) <= kFewLds && tokens * k <= 16384;
+}
+
+// The same for a few hundred tokens, 16 at a time: at most two workgroups a CU, and
+// rows that stay in registers.  Measured against quantise + multiply (aligned rows)
+// or lay out + quantise + multiply: 200 x 1088 x 1088 7.9 / 11.0 us, bf16 7.8 / 11.1;
+// 200 x 1003 x 333 9.9 / 13.7; 4000 x 1088 x 51 8.4 / 13.9; beyond the limits 512 x
+// 1088 x 1088 bf16 14.3 / 11.1, 200 x 4032 x 1024 30 / 15.8.
+bool mid(int64_t tokens, int64_t k, int64_t n) {
+  return tokens > kFewTokens && k <= 1536 && (tokens + 15) / 16 * ((n + 63) / 64) <= 512;
 }
 
 // Tokens of one quantise + multiply round: their integers stay below 1 GiB, which
@@ -694,24 +784,23 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
   g.out = a.out; g.out_row = a.out_row;
   g.tokens = a.tokens; g.n = a.n;
   if (a.tokens <= kFewTokens) {
-    const bool al = a.k % 16 == 0 && a.w_row % 16 == 0 && (uintptr_t)a.w % 16 == 0;
-    const int64_t lds = a.tokens * (kp + 16);
     const dim3 grid((a.n + 15) / 16);
     if (fused(a.tokens, a.k)) {
-      if (al) hipLaunchKernelGGL((int8_few_kernel<T, true, true>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
-      else hipLaunchKernelGGL((int8_few_kernel<T, true, false>), grid, dim3(256), (unsigned)lds, s, g, a.x, a.x_row, a.k);
+      hipLaunchKernelGGL((int8_few_kernel<T, true>), grid, dim3(256), (unsigned)(a.tokens * (kp + 16)), s, g, a.x, a.x_row, a.k);
     } else {
       launch_quant_rows<T>(a, kp, q, qs, s);
-      if (al) hipLaunchKernelGGL((int8_few_kernel<T, false, true>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
-      else hipLaunchKernelGGL((int8_few_kernel<T, false, false>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
+      hipLaunchKernelGGL((int8_few_kernel<T, false>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
     }
     return;
   }
-  // Many rows of whole 16-byte pieces, two workgroups' integers in a CU's LDS (K up to 1216), 32-bit offsets.
-  constexpr int V = kVec<T>;
-  const bool al = a.k % V == 0 && (uintptr_t)a.x % 16 == 0 && a.x_row % V == 0;
+  if (mid(a.tokens, a.k, a.n)) {
+    const dim3 grid((unsigned)((a.tokens + 15) / 16), (unsigned)((a.n + 63) / 64));
+    hipLaunchKernelGGL((int8_mid_kernel<T>), grid, dim3(256), (unsigned)(16 * (kp + 16)), s, g, a.x, a.x_row, a.k);
+    return;
+  }
+  // Many tokens, two workgroups' integers in a CU's LDS (K up to 1216), 32-bit offsets.
   const int64_t n64 = pad64(a.n);
-  if (a.tokens >= kGroupTokens && al && kp * kGroup <= kGroupLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
+  if (a.tokens >= kGroupTokens && kp * kGroup <= kGroupLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
     hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, wp);
     g.w = wp;
     g.w_bytes = n64 * kp;
@@ -724,8 +813,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
   const bool four = a.k % 4 == 0 && a.w_row % 4 == 0 && (uintptr_t)a.w % 4 == 0;
   if (a.tokens >= kPanelTokens || !four || a.w_row % 16 || (uintptr_t)a.w % 16 || g.w_bytes > 0x7fffffff) {
     const dim3 grid((a.n + 15) / 16, (unsigned)(kp / 64));
-    if (four) hipLaunchKernelGGL((panels_kernel<true>), grid, dim3(256), 0, s, a.w, a.w_row, a.n, a.k, wp);
-    else hipLaunchKernelGGL((panels_kernel<false>), grid, dim3(256), 0, s, a.w, a.w_row, a.n, a.k, wp);
+    hipLaunchKernelGGL(panels_kernel, grid, dim3(256), 0, s, a.w, a.w_row, a.n, a.k, wp);
     g.w = wp;
     g.w_row = 64;
     g.w_panel = (int64_t)a.n * 64;
@@ -748,7 +836,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
 
 int64_t int8_workspace(int64_t tokens, int64_t k, int64_t n) {
   if (tokens <= 0 || k <= 0 || n <= 0) return 0;
-  if (fused(tokens, k)) return 0;
+  if (fused(tokens, k) || mid(tokens, k, n)) return 0;
   const int64_t most = round_tokens(tokens, k);
   return pad256(most * 4) + pad256(most * pad64(k)) + pad256(pad64(n) * pad64(k));
 }
