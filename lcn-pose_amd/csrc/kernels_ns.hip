@@ -32,6 +32,7 @@
 // 8-byte piece of the (row j, contraction i) form, and the other form is
 // transposed through LDS.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "ops_common.h"
@@ -52,8 +53,10 @@ struct NsPlan {
   int64_t xplane, aplane;   // bytes of a plane
   int64_t x[2], a, b;       // Xr hi, Xr lo, Xc hi, Xc lo (twice); A hi, lo; B hi, lo
   int64_t stride;
+  int slices;               // of K in the Gram product
+  int64_t parts;            // bytes of its partial sums, all matrices
 };
-NsPlan make_plan(int64_t rows, int64_t cols) {
+NsPlan make_plan(int64_t batch, int64_t rows, int64_t cols) {
   NsPlan p;
   p.m = (int)std::min(rows, cols);
   p.n = (int)std::max(rows, cols);
@@ -66,6 +69,15 @@ NsPlan make_plan(int64_t rows, int64_t cols) {
   p.a = 8 * p.xplane;
   p.b = p.a + 2 * p.aplane;
   p.stride = p.b + 2 * p.aplane;
+  // A 64 x 64 tile goes through 32 of K in 0.2 us; parts of K cost 5 us for their
+  // launch and sums, so they are taken where they shorten the product by 40 stages
+  // and more: one 333 x 7000 327 -> 194 us, one 140 x 4000 204 -> 139.
+  const int64_t c = (p.m + 63) / 64, tiles = batch * c * (c + 1) / 2;
+  const int stages = p.np / 32;
+  int slices = (int)std::min<int64_t>(256 / tiles, stages / 8);
+  if (slices > 1) slices = (stages + (stages + slices - 1) / slices - 1) / ((stages + slices - 1) / slices);  // none empty
+  p.slices = slices > 1 && stages - stages / slices >= 40 ? slices : 1;
+  p.parts = p.slices > 1 ? p.slices * tiles * 16384 : 0;
   return p;
 }
 
@@ -236,7 +248,9 @@ __device__ __forceinline__ void store_some(void* p, int64_t o, const float (&v)[
 }
 
 // ---- the three products --------------------------------------------------------------------
-enum { kGram = 0, kSquare = 1, kUpdate = 2, kFinal = 3 };
+// kPart, kJoin: a Gram matrix of few tiles and long K in two launches, fp32 sums of
+// parts of K by different workgroups, then their total
+enum { kGram = 0, kSquare = 1, kUpdate = 2, kFinal = 3, kPart = 4, kJoin = 5 };
 
 struct NsProd {
   const char* P; const char* Q;       // hi planes of matrix 0; lo planes follow at p_lo / q_lo
@@ -248,6 +262,7 @@ struct NsProd {
   const char* E; int64_t e_lo;        // kSquare: A (= Q), in (row j, contraction i) form
   char* Y; int64_t y_lo;              // result in (row j, contraction i) form
   char* Z; int64_t z_lo;              // result in (row i, contraction j) form
+  float* part; int slices;            // kPart, kJoin: [slice of K][tile][4 waves][16][64]
   float f, e;                         // result = f * sum (+ e * E, + a on the diagonal: kSquare), in the stored forms' scales
 };
 
@@ -271,9 +286,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 #define NS_BUF(I) ((I) % R == 0 ? l0 : (I) % R == 1 ? l1 : (I) % R == 2 ? l2 : l3)
   // The whole tiles of all matrices come first, then those with fewer row blocks
   // of either operand.
-  const int nwhole = g.whole * (int)a.batch;
-  const bool rest = (int)blockIdx.x >= nwhole;
-  const int id = rest ? xcd_remap(blockIdx.x - nwhole, gridDim.x - nwhole) : xcd_remap(blockIdx.x, nwhole);
+  const int nwhole = g.whole * (int)a.batch, ntiles = MODE == kPart ? gridDim.x / g.slices : gridDim.x;
+  const int slice = MODE == kPart ? blockIdx.x / ntiles : 0, block = MODE == kPart ? blockIdx.x % ntiles : blockIdx.x;
+  const bool rest = block >= nwhole;
+  const int id = rest ? xcd_remap(block - nwhole, ntiles - nwhole) : xcd_remap(block, nwhole);
   const int mat = id / (rest ? g.rest : g.whole);
   int t = id - mat * (rest ? g.rest : g.whole);
   int ti, tj;
@@ -289,7 +305,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       while ((ti + 1) * (ti + 2) <= t) ++ti;
       tj = t - ti * (ti + 1);
     }
-  } else if constexpr (MODE == kGram || MODE == kSquare) {  // lower triangle, ti >= tj, row after row
+  } else if constexpr (MODE != kUpdate && MODE != kFinal) {  // lower triangle, ti >= tj, row after row
     if (rest) t += g.whole;
     ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > t) --ti;
@@ -320,16 +336,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   const __amdgpu_buffer_rsrc_t rql = __builtin_amdgcn_make_buffer_rsrc((void*)(Qm + g.q_lo + (int64_t)qb * rb_bytes), 0, rb_bytes, 0x00020000);
   const int vo = lane * 16;
   // stage layout: P hi | P lo | Q hi | Q lo, row blocks x 1 KB pieces of K
+  const int all = g.K / (16 * KK), share = MODE == kPart ? (all + g.slices - 1) / g.slices : all;
+  const int first = slice * share, nk = MODE == kJoin ? 0 : min(share, all - first);  // this workgroup's stages
   auto stage = [&](int ks, char* buf) {
     char* d = buf + w * 1024;
-    const int so = ks * (1024 * KK) + sk;
+    const int so = (first + ks) * (1024 * KK) + sk;
     NS_LDS(rph, vo, so, d);
     NS_LDS(rpl, vo, so, d + kP);
     NS_LDS(rqh, vo, so, d + 2 * kP);
     if constexpr (NI == NJ) NS_LDS(rql, vo, so, d + 2 * kP + kQ);
   };
   f32x16 acc[NI][NJ] = {}, cr = {};  // cr: 64 x 64 alternates between two sums, which do not wait for each other
-  const int nk = g.K / (16 * KK);
   struct Frag { half8 ph[NI * KK], pl[NI * KK], qh[NJ * KK], ql[NJ * KK]; };  // [row block][piece of K]
   auto fetch = [&](const char* buf, Frag& f) {
     const char *p = buf + wi * NI * KK * 1024 + vo, *q = buf + 2 * kP + wj * NJ * KK * 1024 + vo;
@@ -393,7 +410,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
       for (int i = 0; i < R; ++i) step(ks + i, NS_BUF(i), NS_BUF(i + 1), f[i & 1], f[(i + 1) & 1], true, true);
       ks += R;
     } while (ks + 2 * R <= nk);
-  } else {
+  } else if (MODE != kJoin) {
 #pragma unroll
     for (int i = 0; i < R; ++i)
       if (i < nk) stage(i, NS_BUF(i));
@@ -408,6 +425,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
   }
 #undef NS_BUF
   if constexpr (NI == 1) acc[0][0] += cr;
+  if constexpr (MODE == kPart || MODE == kJoin) {
+    const int64_t tile = (int64_t)mat * (g.whole + g.rest) + t, tiles = (int64_t)(g.whole + g.rest) * a.batch;
+    float* sums = g.part + (tile * 4 + w) * 1024 + lane;
+    if constexpr (MODE == kPart) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sums[slice * tiles * 4096 + e * 64] = acc[0][0][e];
+      return;
+    }
+    constexpr int kAhead = 4;
+    for (int q0 = 0; q0 < g.slices; q0 += kAhead) {  // in their order
+      float v[kAhead][16];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[q][e] = q0 + q < g.slices ? sums[(q0 + q) * tiles * 4096 + e * 64] : 0.f;
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[0][0][e] += v[q][e];
+    }
+  }
   __syncthreads();
   // epilogue, one 32 x 32 block at a time; the wave transposes in a ring buffer of its own
   unsigned* tr = (unsigned*)(w == 0 ? l0 : w == 1 ? l1 : w == 2 ? l2 : l3);
@@ -523,7 +561,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
     }
 }
 
-// ---- matrices with a short side of at most 128 ---------------------------------------------
+// ---- matrices with a short side of at most 64 ----------------------------------------------
 // The short side's Gram matrix fits into LDS, so a workgroup does a whole step
 // for its own columns of X: A (from all workgroups' partial sums), B = a I + b A +
 // c A A (every workgroup for itself), X <- B X, and the next Gram matrix's partial
@@ -553,13 +591,28 @@ struct ThinGeo {
   static_assert(MT * MT % NW == 0 && MT * WT % NW == 0 && M * W % kThreads == 0 && kImage / 2 % (16 * kThreads) == 0, "");
 };
 template <int MB, int WB, int NW>
-ThinPlan make_thin(int64_t rows, int64_t cols) {
+ThinPlan make_thin(int64_t batch, int64_t rows, int64_t cols) {
   using G = ThinGeo<MB, WB, NW>;
   ThinPlan p;
   p.m = (int)std::min(rows, cols);
   p.n = (int)std::max(rows, cols);
   p.chunks = (p.n + G::W - 1) / G::W;
-  p.slabs = std::min(p.chunks, 48);
+  // Slabs of a matrix, equal shares: the more, the fewer chunks each, but each reads
+  // all partial sums of a step and squares them (about a chunk's time), and past a
+  // workgroup a CU (M 32: two, of four waves) they take turns.  Measured: 14 x 48 x 4253 (34 chunks) 34 / 17 slabs 174 / 130 us;
+  // 54 x 57 x 2789 (22) 22 / 8 / 6 / 4: 363 / 258 / 262 / 225; 132 x 54 x 1902 (15)
+  // 15 / 3 / 2 / 1: 515 / 300 / 385 / 363; one 64 x 7000 (55) 28 / 19: 77 / 85; M 32:
+  // 72 x 29 x 3946 (31) 11 / 8 / 7: 228 / 223 / 216, 51 x 21 x 2150 (17) 17 / 9: 111 / 99.
+  float best = 1e30f;
+  for (int each = 1; each <= p.chunks; each = each < 32 || each == p.chunks ? each + 1 : p.chunks) {
+    const int slabs = (p.chunks + each - 1) / each;
+    const float wgs = (float)slabs * batch;
+    const float cost = (MB == 1 ? std::max(1.f, wgs / 512) : std::ceil(wgs / 256)) * (each + 0.08f * slabs + 1);
+    if (slabs <= 48 && cost < best) {
+      best = cost;
+      p.slabs = slabs;
+    }
+  }
   p.grams = 0;
   p.images = 2 * (int64_t)p.slabs * G::kGram;
   p.stride = p.chunks == 1 ? 0 : p.images + (int64_t)p.chunks * G::kImage;
@@ -850,7 +903,7 @@ int norm_parts(const NsArgs& a) {
 template <int MB, int WB, int NW, int T, bool kMuon>
 void launch_thin(const NsArgs& a, void* workspace, hipStream_t s) {
   using G = ThinGeo<MB, WB, NW>;
-  const ThinPlan p = make_thin<MB, WB, NW>(a.rows, a.cols);
+  const ThinPlan p = make_thin<MB, WB, NW>(a.batch, a.rows, a.cols);
   double* part = (double*)workspace;
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
   if (p.chunks == 1) {
@@ -867,17 +920,19 @@ void launch_thin(const NsArgs& a, void* workspace, hipStream_t s) {
   hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kLast>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
 }
 
-// The path of a matrix by its sides: short side at most 64 with chunks of 64
-// columns where one holds the long side, else of 128; at most 128 with chunks of
-// 64; larger ones in tiles.  Waves, measured with 4 / 8 / 16: 175 x 64 x 64
-// 20 / 15 / 15 us (4 000 of them 176 / 156 / 180), a step of 51 x 1088
-// 10.4 / 7.8 / 7.2, of 128 x 1000 35 / 22 / 20.
-enum { kThinSmall, kThin64, kThin128, kTiled };
-constexpr int kWavesSmall = 8, kWaves64 = 16, kWaves128 = 16;
+// The path of a matrix by its sides: short side at most 64 in one launch where the
+// long side is at most 64 too, else in chunks of 128 columns, with a Gram matrix of
+// 32 x 32 or 64 x 64; larger ones in tiles.  Measured, M 32 / 64: one 20 x 1088 33 /
+// 43 us, 58 x 30 x 528 54 / 77; a Gram matrix of 128 x 128 in LDS / tiles: one 128 x
+// 1000 108 / 100 us, 96 x 71 x 846 261 / 230.  Waves, measured with 4 / 8 / 16:
+// 175 x 64 x 64 20 / 15 / 15 us (4 000 of them 176 / 156 / 180), a step of 51 x 1088
+// 10.4 / 7.8 / 7.2.
+enum { kThinSmall, kThin32, kThin64, kTiled };
+constexpr int kWavesSmall = 8, kWaves32 = 4, kWaves64 = 16;
 int path_of(int64_t rows, int64_t cols) {
   const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
-  if (m <= 64) return n <= 64 ? kThinSmall : kThin64;
-  return m <= 128 ? kThin128 : kTiled;
+  if (n <= 64) return kThinSmall;
+  return m <= 32 ? kThin32 : m <= 64 ? kThin64 : kTiled;
 }
 
 // Tiles of 128 x 128, 128 x 64 (symmetric products) or 64 x 64.  A launch lasts as
@@ -935,12 +990,13 @@ template <int T, bool kMuon>
 void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
   switch (path_of(a.rows, a.cols)) {
     case kThinSmall: return launch_thin<2, 2, kWavesSmall, T, kMuon>(a, workspace, s);
+    case kThin32: return launch_thin<1, 4, kWaves32, T, kMuon>(a, workspace, s);
     case kThin64: return launch_thin<2, 4, kWaves64, T, kMuon>(a, workspace, s);
-    case kThin128: return launch_thin<4, 2, kWaves128, T, kMuon>(a, workspace, s);
   }
-  const NsPlan p = make_plan(a.rows, a.cols);
+  const NsPlan p = make_plan(a.batch, a.rows, a.cols);
   double* part = (double*)workspace;
   char* ws = (char*)workspace + a.batch * kNormParts * 8;
+  float* parts_at = (float*)(ws + a.batch * p.stride);
   const int parts = norm_parts(a);
   launch_norm<T, kMuon>(a, parts, part, s);
   hipLaunchKernelGGL((ns_init_kernel<T, kMuon>), dim3((p.mp / 32) * ((p.np / 32 + kInit - 1) / kInit), (unsigned)a.batch), dim3(256), 0, s, a, p, parts, part, ws);
@@ -957,7 +1013,18 @@ void launch_ns_t(const NsArgs& a, void* workspace, hipStream_t s) {
     g.Y = g.Z = ws + p.a;
     g.y_lo = g.z_lo = p.aplane;
     g.f = kSa / (kSx * kSx);
-    launch_prod<kGram, kOpF32>(g, a, p, s);
+    if (p.slices > 1) {
+      const int c = p.mp / 64, odd = p.mp % 64 != 0;
+      g.whole = c * (c + 1) / 2;
+      g.rest = odd * (c + 1);
+      g.part = parts_at;
+      g.slices = p.slices;
+      const unsigned tiles = (unsigned)((g.whole + g.rest) * a.batch);
+      hipLaunchKernelGGL((ns_prod_kernel<kPart, kOpF32, 1, 1>), dim3(tiles * p.slices), dim3(256), 0, s, g, a, p);
+      hipLaunchKernelGGL((ns_prod_kernel<kJoin, kOpF32, 1, 1>), dim3(tiles), dim3(256), 0, s, g, a, p);
+    } else {
+      launch_prod<kGram, kOpF32>(g, a, p, s);
+    }
     // B = a I + b A + c A A
     g.P = g.Q = g.E = ws + p.a;
     g.p_lo = g.q_lo = g.e_lo = p.aplane;
@@ -988,10 +1055,13 @@ int64_t ns_workspace(int64_t batch, int64_t rows, int64_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
   int64_t stride = 0;
   switch (path_of(rows, cols)) {
-    case kThinSmall: stride = make_thin<2, 2, kWavesSmall>(rows, cols).stride; break;
-    case kThin64: stride = make_thin<2, 4, kWaves64>(rows, cols).stride; break;
-    case kThin128: stride = make_thin<4, 2, kWaves128>(rows, cols).stride; break;
-    default: stride = make_plan(rows, cols).stride;
+    case kThinSmall: stride = make_thin<2, 2, kWavesSmall>(batch, rows, cols).stride; break;
+    case kThin32: stride = make_thin<1, 4, kWaves32>(batch, rows, cols).stride; break;
+    case kThin64: stride = make_thin<2, 4, kWaves64>(batch, rows, cols).stride; break;
+    default: {
+      const NsPlan p = make_plan(batch, rows, cols);
+      return batch * (kNormParts * 8 + p.stride) + p.parts;
+    }
   }
   return batch * (kNormParts * 8 + stride);
 }

@@ -78,6 +78,18 @@ def test_orthogonalize_hidden_and_large_batch():
     close(ops.orthogonalize(g), polynomial(g), torch.float32)
 
 
+# many matrices, of which a workgroup takes several chunks of columns; and few with a long contraction, whose Gram
+# matrix is summed in slices
+@pytest.mark.parametrize("shape", [(300, 40, 500), (700, 300, 20), (90, 64, 1300), (2, 333, 5000), (3, 5003, 97), (1, 65, 2111), (40, 66, 70)])
+def test_orthogonalize_batches_and_long_sides(shape):
+    g = gradient(shape, torch.float32, seed=shape[0])
+    close(ops.orthogonalize(g), polynomial(g), torch.float32)
+    p, m = torch.zeros_like(g), gradient(shape, torch.float32, seed=1)
+    want = muon_reference(p, m, g, 0.01, 0.95, True, 0.0, 1.0)
+    ops.muon_update(p, m, g, lr=0.01, scale=1.0)
+    muon_close(p, m, *want, 0.01, 1.0)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(192, 192), (48, 40)])
 def test_orthogonalize_low_rank(dtype, shape):
