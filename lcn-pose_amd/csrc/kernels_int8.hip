@@ -95,6 +95,7 @@ __device__ __forceinline__ v4i weights16(const int8_t* p, int left, const int8_t
   }
   return v;
 }
+
 // One wave a row: largest magnitude, then the integers, rows padded to kp with
 // zeros.  A lane keeps up to kRegs pieces in registers between the two passes; what
 // is past them is read again (from L2).  Bound by memory: 65 536 x 1088 fp32 in 60 us

@@ -599,10 +599,11 @@ ThinPlan make_thin(int64_t batch, int64_t rows, int64_t cols) {
   p.chunks = (p.n + G::W - 1) / G::W;
   // Slabs of a matrix, equal shares: the more, the fewer chunks each, but each reads
   // all partial sums of a step and squares them (about a chunk's time), and past a
-  // workgroup a CU (M 32: two, of four waves) they take turns.  Measured: 14 x 48 x 4253 (34 chunks) 34 / 17 slabs 174 / 130 us;
-  // 54 x 57 x 2789 (22) 22 / 8 / 6 / 4: 363 / 258 / 262 / 225; 132 x 54 x 1902 (15)
-  // 15 / 3 / 2 / 1: 515 / 300 / 385 / 363; one 64 x 7000 (55) 28 / 19: 77 / 85; M 32:
-  // 72 x 29 x 3946 (31) 11 / 8 / 7: 228 / 223 / 216, 51 x 21 x 2150 (17) 17 / 9: 111 / 99.
+  // workgroup a CU (M 32: two, of four waves) they take turns.  Measured: 14 x 48 x
+  // 4253 (34 chunks) 34 / 17 slabs 174 / 130 us; 54 x 57 x 2789 (22) 22 / 8 / 6 / 4:
+  // 363 / 258 / 262 / 225; 132 x 54 x 1902 (15) 15 / 3 / 2 / 1: 515 / 300 / 385 / 363;
+  // one 64 x 7000 (55) 28 / 19: 77 / 85; M 32: 72 x 29 x 3946 (31) 11 / 8 / 7: 228 /
+  // 223 / 216, 51 x 21 x 2150 (17) 17 / 9: 111 / 99.
   float best = 1e30f;
   for (int each = 1; each <= p.chunks; each = each < 32 || each == p.chunks ? each + 1 : p.chunks) {
     const int slabs = (p.chunks + each - 1) / each;
