@@ -80,7 +80,9 @@ bool overlap(const View& a, const View& b) {
 bool same_place(const View& a, const View& b) {
   return a.p == b.p && a.bytes == b.bytes && (a.batch == 1 || a.s_batch == b.s_batch) && (a.rows == 1 || a.s_row == b.s_row);
 }
+// (a null block: the call needs none)
 bool in_block(const View& v, const void* block, int64_t bytes) {
+  if (!block) return false;
   const uint64_t b = (uint64_t)(uintptr_t)block;
   return v.begin() < b + (uint64_t)bytes && b < v.end();
 }

@@ -90,8 +90,9 @@ def _int8(lib, **kw):
     (dict(w=None), "null"), (dict(s=None), "null"), (dict(out=None), "null"), (dict(x=A + 2), "aligned"),
     (dict(s=C + 2), "aligned"), (dict(b=C + 1), "aligned"), (dict(xr=-1), "strides"), (dict(wr=-4), "strides"),
     (dict(orow=15), "rows overlap"), (dict(out=A + 16), "overlaps an input"), (dict(out=B), "overlaps an input"),
-    (dict(out=C), "overlaps an input"), (dict(b=4 << 32), "overlaps an input"), (dict(ws=None), "workspace"),
-    (dict(wsb=16), "needed"), (dict(w=WS + 16), "workspace overlaps"),
+    (dict(out=C), "overlaps an input"), (dict(b=4 << 32), "overlaps an input"),
+    (dict(k=2048, xr=2048, wr=2048, ws=None), "null workspace"), (dict(k=2048, xr=2048, wr=2048, ws=WS + 8), "256-byte"),
+    (dict(k=2048, xr=2048, wr=2048, wsb=16), "needed"), (dict(k=2048, xr=2048, wr=2048, w=WS + 16), "workspace overlaps"),
 ])
 def test_int8_linear_refuses(lib, kw, word):
     assert _int8(lib, **kw) == -1
