@@ -619,22 +619,25 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
 }
 
 // ---- up to some hundred tokens ---------------------------------------------------------------
-// A workgroup takes 16 tokens x 64 channels: it quantises the tokens into LDS, four
-// rows a wave with all their loads in flight, each of the n / 64 workgroups anew
-// (they come from L2), and a wave multiplies them by 16 channels, whose weights
-// are asked for before the quantisation starts.  One launch, no workspace.  Bound
-// by latency (the rows, their largest magnitude, the weights of the second half of
-// K): 200 x 1088 x 1088 in 7.5 us.
-constexpr int kMidAhead = 6;  // 64-byte pieces of K in flight
+// A workgroup takes 16 tokens x 64 channels: each of its 16 waves quantises a token
+// into LDS, each of the n / 64 workgroups anew (they come from L2), then multiplies
+// the 16 tokens by 16 channels over every fourth 64-byte piece of K, whose weights
+// are asked for before the quantisation starts; the four sums of a block meet in
+// LDS.  One launch, no workspace.  Bound by latency (the rows, their largest
+// magnitude, the weights): 200 x 1088 x 1088 in 6.3 us, 8.8 with 4 waves, 6.9 with 8.
+constexpr int kMidWaves = 16;
 template <int T>
-__global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
+__global__ __launch_bounds__(64 * kMidWaves) __attribute__((amdgpu_waves_per_eu(8))) void int8_mid_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int kKs = kMidWaves / 4, kRows = 16 / kMidWaves;  // waves that share 16 channels, rows of a wave
+  constexpr int kMidAhead = 4;  // 64-byte pieces of K of a wave in flight
   __shared__ float qs[16];
+  __shared__ int sums[kKs - 1][4][4][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kp = (int)g.kp, nk = kp / 64, pitch = kp + 16;
   const int64_t t0 = (int64_t)blockIdx.x * 16;
   const int rows = (int)min((int64_t)16, g.tokens - t0);
-  const int c16 = lane & 15, kq = lane >> 4, n0 = blockIdx.y * 64 + w * 16;
+  const int c16 = lane & 15, kq = lane >> 4, n0 = blockIdx.y * 64 + (w & 3) * 16, part = w >> 2;
   // channels past the last repeat it, K past its end meets zeros of the tokens
   const int8_t* wrow = g.w + (int64_t)min(n0 + c16, g.n - 1) * g.w_row;
   const int8_t* wend = g.w + g.w_bytes;
@@ -644,10 +647,10 @@ __global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* _
   };
   v4i wv[kMidAhead];
 #pragma unroll
-  for (int i = 0; i < kMidAhead; ++i) wv[i] = weights(i);
+  for (int i = 0; i < kMidAhead; ++i) wv[i] = weights(part + kKs * i);
   {
     // the first kRegs pieces of four rows stay in registers
-    constexpr int V = kVec<T>, kRegs = T == kOpF32 ? 5 : 3, kRows = 4;
+    constexpr int V = kVec<T>, kRegs = T == kOpF32 ? 5 : 3;
     const int whole = k / V, padded = kp / V;
     int64_t r[kRows];
     v4u keep[kRows][kRegs], tail[kRows];
@@ -655,7 +658,7 @@ __global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* _
     bool bad[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      r[j] = (t0 + min(w * 4 + j, rows - 1)) * x_row;
+      r[j] = (t0 + min(w * kRows + j, rows - 1)) * x_row;
       tail[j] = v4u{0, 0, 0, 0};
       if (k % V) tail[j] = tail_piece<T>(x, r[j] + (int64_t)whole * V, k % V, lane);
 #pragma unroll
@@ -672,13 +675,15 @@ __global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* _
 #pragma unroll
       for (int j = 0; j < kRows; ++j) see_piece<T>(row_piece<T, false>(x, r[j], c, whole, tail[j]), top[j], bad[j]);
     float factor[kRows];
-    char* o = lds + w * 4 * pitch;
+    char* o = lds + w * kRows * pitch;
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       float s;
       wave_top(top[j], bad[j]);
       row_scale(top[j], bad[j], factor[j], s);
-      if (lane == 0) qs[w * 4 + j] = s;
+      if (lane == 0) qs[w * kRows + j] = s;
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) asm volatile("" : "+v"(keep[j][i]));  // unpacked anew, not kept as floats
 #pragma unroll
       for (int i = 0; i < kRegs; ++i)
         if (lane + 64 * i < padded) put_piece<T>(o + j * pitch + (lane + 64 * i) * V, keep[j][i], factor[j], bad[j]);
@@ -690,14 +695,24 @@ __global__ __launch_bounds__(256) void int8_mid_kernel(Int8Gemm g, const void* _
   __syncthreads();
   v4i acc = {0, 0, 0, 0};
   const char* a = lds + c16 * pitch + kq * 16;
-  for (int ks = 0; ks < nk; ks += kMidAhead) {
+  for (int ks = part; ks < nk; ks += kKs * kMidAhead) {
 #pragma unroll
     for (int i = 0; i < kMidAhead; ++i) {
-      if (ks + i >= nk) break;
-      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(a + (ks + i) * 64), wv[i], acc, 0, 0, 0);
-      wv[i] = weights(ks + i + kMidAhead);
+      const int p = ks + kKs * i;
+      if (p >= nk) break;
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(a + p * 64), wv[i], acc, 0, 0, 0);
+      wv[i] = weights(p + kKs * kMidAhead);
     }
   }
+  if (part)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[part - 1][w & 3][e][lane] = acc[e];
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int q = 0; q + 1 < kKs; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += sums[q][w & 3][e][lane];
   // lane holds tokens 4 kq .. 4 kq + 3 of channel c16
   const int n = n0 + c16;
   if (n < g.n) {
@@ -757,11 +772,11 @@ bool fused(int64_t tokens, int64_t k) {
 
 // The same for a few hundred tokens, 16 at a time: at most two workgroups a CU, and
 // rows that stay in registers.  Measured against quantise + multiply (aligned rows)
-// or lay out + quantise + multiply: 200 x 1088 x 1088 7.9 / 11.0 us, bf16 7.8 / 11.1;
-// 200 x 1003 x 333 9.9 / 13.7; 4000 x 1088 x 51 8.4 / 13.9; beyond the limits 512 x
-// 1088 x 1088 bf16 14.3 / 11.1, 200 x 4032 x 1024 30 / 15.8.
+// or lay out + quantise + multiply, in a graph: 200 x 1088 x 1088 6.3 / 8.8 us, 480 x
+// 1088 x 1088 8.6 / 8.9, 200 x 1003 x 333 7.8 / 10.6, 4000 x 1088 x 51 6.4 / 13.5;
+// beyond the limit 512 x 1088 x 1088 11.4 / 9.1; with rows of 4032 read twice 30 / 16.
 bool mid(int64_t tokens, int64_t k, int64_t n) {
-  return tokens > kFewTokens && k <= 1536 && (tokens + 15) / 16 * ((n + 63) / 64) <= 512;
+  return !fused(tokens, k) && k <= 1536 && (tokens + 15) / 16 * ((n + 63) / 64) <= 512;
 }
 
 // Tokens of one quantise + multiply round: their integers stay below 1 GiB, which
@@ -784,6 +799,11 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
   g.ws = a.w_scale; g.bias = a.bias;
   g.out = a.out; g.out_row = a.out_row;
   g.tokens = a.tokens; g.n = a.n;
+  if (mid(a.tokens, a.k, a.n)) {
+    const dim3 grid((unsigned)((a.tokens + 15) / 16), (unsigned)((a.n + 63) / 64));
+    hipLaunchKernelGGL((int8_mid_kernel<T>), grid, dim3(64 * kMidWaves), (unsigned)(16 * (kp + 16)), s, g, a.x, a.x_row, a.k);
+    return;
+  }
   if (a.tokens <= kFewTokens) {
     const dim3 grid((a.n + 15) / 16);
     if (fused(a.tokens, a.k)) {
@@ -792,11 +812,6 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
       launch_quant_rows<T>(a, kp, q, qs, s);
       hipLaunchKernelGGL((int8_few_kernel<T, false>), grid, dim3(256), 0, s, g, a.x, a.x_row, a.k);
     }
-    return;
-  }
-  if (mid(a.tokens, a.k, a.n)) {
-    const dim3 grid((unsigned)((a.tokens + 15) / 16), (unsigned)((a.n + 63) / 64));
-    hipLaunchKernelGGL((int8_mid_kernel<T>), grid, dim3(256), (unsigned)(16 * (kp + 16)), s, g, a.x, a.x_row, a.k);
     return;
   }
   // Many tokens, two workgroups' integers in a CU's LDS (K up to 1216), 32-bit offsets.
