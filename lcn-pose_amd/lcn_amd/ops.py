@@ -134,7 +134,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
     dt = _dtype(g, "g")
     n, r, c, sb, sr = _matrices(g, "g")
     if out is None:
-        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        out = g.new_empty(g.shape)
     else:
         _tensor(out, "out", g.device)
         _expect(out.shape == g.shape and out.dtype == g.dtype, "out differs from g in shape or type")
@@ -234,7 +234,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias
     x2 = x if len(shape) == 2 else _rows(x, "x")
     tokens = x2.shape[0]
     if out is None:
-        out2 = torch.empty((tokens, n), dtype=x.dtype, device=dev)
+        out2 = x.new_empty(tokens, n)
         out = out2 if len(shape) == 2 else out2.view(shape[:-1] + (n,))
     else:
         _tensor(out, "out", dev)
