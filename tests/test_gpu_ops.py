@@ -275,7 +275,8 @@ def int8_close(got, x, w, s, b):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("t,k,n", [(1, 1, 1), (1, 64, 64), (1, 1088, 1088), (2, 51, 1088), (3, 1003, 333), (15, 16, 17), (16, 128, 128),
                                    (17, 80, 31), (31, 200, 64), (33, 34, 1088), (64, 64, 129), (65, 144, 127), (127, 1088, 51),
-                                   (128, 65, 256), (129, 63, 130), (200, 1088, 1088), (777, 1003, 333), (1000, 96, 16), (1030, 1088, 340)])
+                                   (128, 65, 256), (129, 63, 130), (200, 1088, 1088), (777, 1003, 333), (1000, 96, 16), (1030, 1088, 340), (16, 1088, 70), (13, 2520, 40),
+                                   (200, 1601, 96), (21, 1535, 130), (600, 1087, 1025)])
 def test_int8_linear_shapes(t, k, n, dtype):
     for bias in (True, False):
         x, w, s, b = int8_case(t, k, n, dtype, seed=t + k + n, bias=bias)
