@@ -123,9 +123,11 @@ int lcn_set_dropout(void* handle, float rate, uint64_t seed);
  * momentum takes the place of Adam's m for these weights
  * (lcn_get/set_optimizer_state; their v is not used).  momentum in [0, 1), steps
  * in [1, 64].  LCN_OPT_ADAM (the state after lcn_create) ignores the other
- * arguments.  Replicas of several ranks stay equal: the update follows the
- * all-reduced gradients.  No counterpart in the reference (Adam only,
- * models_att.py:404-409). */
+ * arguments.  A change of kind sets the hidden weights' m and v to zero (one
+ * rule's state is not the other's), so saved state is handed over after it; new
+ * arguments for the same kind keep them.
+ * Replicas of several ranks stay equal: the update follows the all-reduced
+ * gradients.  No counterpart in the reference (Adam only, models_att.py:404-409). */
 enum { LCN_OPT_ADAM = 0, LCN_OPT_MUON = 1 };
 int lcn_set_optimizer(void* handle, int32_t kind, float momentum, int32_t nesterov, float weight_decay,
                       int32_t steps);

@@ -2058,6 +2058,14 @@ extern "C" int lcn_set_optimizer(void* handle, int32_t kind, float momentum, int
     h->mu_decay = weight_decay;
     h->mu_steps = steps;
   }
+  if (kind != h->optimizer) {
+    // m and v of the hidden weights are the other rule's state (Muon's momentum is an
+    // undamped sum, 1 / (1 - beta) gradients, and it leaves v behind): zero, as a
+    // checkpoint of the other optimiser restores
+    for (int k = 1; k <= 2 * h->L; ++k)
+      for (float* state : {h->m, h->v})
+        HIPC(hipMemsetAsync(state + h->wl[k].w_off, 0, (size_t)h->H * h->H * 4, h->stream));
+  }
   h->optimizer = kind;
   for (auto& g : h->graphs) hipGraphExecDestroy(g.exec);
   h->graphs.clear();

@@ -296,7 +296,8 @@ class Network:
 
     def set_optimizer(self, kind: str, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         """The optimiser of the hidden weights from the next step on: "adam", or "muon"
-        (lcn_set_optimizer; every other variable stays with Adam)."""
+        (lcn_set_optimizer; every other variable stays with Adam).  A change of kind starts
+        the hidden weights' optimiser state at zero."""
         if kind not in OPTIMIZERS:
             raise ValueError(f"unknown optimizer {kind!r}, expected one of {sorted(OPTIMIZERS)}")
         self._check(self.lib.lcn_set_optimizer(self.h, OPTIMIZERS[kind], float(momentum), int(bool(nesterov)),
