@@ -188,6 +188,11 @@ def _restore_npz(net, prefix: str):
         if names != [n for n, _, _ in net.param_layout()]:
             raise ValueError(f"checkpoint {path} does not match the model's variables")
         net.set_params(z["params"])
-        net.set_optimizer_state(z["adam_m"], z["adam_v"], int(z["global_step"]),
+        m, v = z["adam_m"], z["adam_v"]
+        for name, off, shape in net.param_layout():
+            if _momentum(net, name):  # Adam's state is not Muon's: it starts at zero
+                k = int(np.prod(shape))
+                m[off:off + k] = v[off:off + k] = 0
+        net.set_optimizer_state(m, v, int(z["global_step"]),
                                 float(z["beta1_power"]), float(z["beta2_power"]))
     return None
