@@ -8,7 +8,8 @@
 Each runs on its tensors' device and torch's current stream of that device,
 returns without synchronising, takes its scratch memory from torch's allocator
 and can be captured into a graph.  There is no CPU path: tensors on the host are
-refused.  A bad argument raises ``ValueError``, a failure of the library
+refused.  None gives derivatives: a tensor that requires a gradient (outside
+``torch.no_grad()``) or carries a forward-mode tangent is refused.  A bad argument raises ``ValueError``, a failure of the library
 ``LcnNativeError``.  cgcnn and the CLIs reach the same kernels through
 ``Network.set_optimizer`` and ``Network.set_precision``.
 """
@@ -18,6 +19,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .native import DTYPE_BF16, DTYPE_F16, DTYPE_F32, LcnNativeError, load_library
 
@@ -65,6 +67,10 @@ def _tensor(t, name: str, device=None) -> torch.Tensor:
         raise ValueError(f"{name} is a negated view: call resolve_neg() on it")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not give: call it under torch.no_grad()")
+    # (the level is -1 outside forward_ad.dual_level(): asked first, it costs less)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent, which this operator does not pass on: call it on "
+                         "forward_ad.unpack_dual(...).primal")
     return t
 
 
