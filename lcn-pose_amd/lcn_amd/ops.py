@@ -74,6 +74,11 @@ def _tensor(t, name: str, device=None) -> torch.Tensor:
     return t
 
 
+# Tensors written through their address: autograd then tells a backward that saved
+# them that they changed, as after torch's own in-place operators.
+_written = torch.autograd.graph.increment_version
+
+
 def _matrices(t: torch.Tensor, name: str):
     """(batch, rows, cols, batch stride, row stride) of a [rows, cols] or [batch, rows, cols] tensor."""
     shape, s = t.shape, t.stride()
@@ -139,7 +144,8 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
     _tensor(g, "g")
     dt = _dtype(g, "g")
     n, r, c, sb, sr = _matrices(g, "g")
-    if out is None:
+    given = out is not None
+    if not given:
         out = g.new_empty(g.shape)
     else:
         _tensor(out, "out", g.device)
@@ -149,6 +155,8 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
     ws, ws_ptr, ws_bytes = _workspace("lcn_orthogonalize_workspace", n, r, c, g.device)
     _check(lib.lcn_orthogonalize(device, _stream(device), dt, n, r, c, g.data_ptr(), sb, sr, out.data_ptr(),
                                  ob, orow, int(steps), _triple(coefficients), eps, ws_ptr, ws_bytes))
+    if given:
+        _written(out)
     return out
 
 
@@ -187,6 +195,7 @@ def muon_update(param: torch.Tensor, momentum: torch.Tensor, grad: torch.Tensor,
     _check(lib.lcn_muon_update(device, _stream(device), dt, n, r, c, param.data_ptr(), pb, pr,
                                momentum.data_ptr(), mb, mr, grad.data_ptr(), gb, gr, lr_value, lr_ptr, scale, beta,
                                int(nesterov), weight_decay, int(steps), _triple(coefficients), eps, ws_ptr, ws_bytes))
+    _written((param, momentum))
 
 
 def quantize_weight(w: torch.Tensor, *, channel_dim: int = 0):
@@ -239,7 +248,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias
         bias_ptr = bias.data_ptr()
     x2 = x if len(shape) == 2 else _rows(x, "x")
     tokens = x2.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         out2 = x.new_empty(tokens, n)
         out = out2 if len(shape) == 2 else out2.view(shape[:-1] + (n,))
     else:
@@ -251,6 +261,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias
     ws, ws_ptr, ws_bytes = _workspace("lcn_int8_linear_workspace", tokens, k, n, dev)
     _check(lib.lcn_int8_linear(device, _stream(device), dt, tokens, k, n, x2.data_ptr(), x2.stride(0), weight.data_ptr(),
                                ws_row, scale.data_ptr(), bias_ptr, out2.data_ptr(), out2.stride(0), ws_ptr, ws_bytes))
+    if given:
+        _written(out)
     return out
 
 
