@@ -276,7 +276,8 @@ int lcn_eval_mpjpe_static(int32_t device, int64_t n, const double* pred, const d
  * LCN_DTYPE_F32, _BF16 or _F16.  Matrices have a contiguous last dimension; strides are in elements
  * and not negative; batch strides are unused with batch 1, row strides with one
  * row.  Operands that would overlap where they must not are LCN_E_ARG, an
- * empty batch is LCN_OK.  Errors: lcn_last_error(NULL).  No counterpart in the
+ * empty batch is LCN_OK.  Errors: lcn_last_error(NULL); a HIP error that an
+ * earlier call left pending on the thread is cleared.  No counterpart in the
  * reference (its optimiser is Adam, models_att.py:404-409; it predicts in
  * float32, :79-132). */
 

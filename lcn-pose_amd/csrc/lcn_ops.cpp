@@ -23,7 +23,9 @@ int fail(const char* who, const std::string& what, int code = LCN_E_ARG) {
   return code;
 }
 
-// the operator runs on `device`; the calling thread's current device is put back
+// The operator runs on `device`; the calling thread's current device is put back.
+// HIP keeps a thread's last error until it is asked for: what an earlier call left
+// (or a refused device, here) is taken away, so that `launched` sees the launches only.
 struct DeviceGuard {
   int before = -1;
   hipError_t err = hipSuccess;
@@ -31,6 +33,7 @@ struct DeviceGuard {
     err = hipGetDevice(&before);
     if (err == hipSuccess && before != device) err = hipSetDevice(device);
     else before = -1;
+    (void)hipGetLastError();
   }
   ~DeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
 };
