@@ -26,6 +26,7 @@ __host__ __device__ inline int64_t pad256(int64_t v) { return (v + 255) / 256 * 
 
 constexpr int64_t kPanelTokens = 1024;
 constexpr int64_t kGroupTokens = 16384;  // one workgroup of 64 a CU
+constexpr int64_t kGroupMost = (int64_t)1 << 29;  // of a launch, whose threads are counted in 32 bits
 
 // largest magnitude of a wave's values, and whether one is an infinity or a NaN
 __device__ __forceinline__ void wave_top(float& top, bool& bad) {
@@ -820,7 +821,12 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
     hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, wp);
     g.w = wp;
     g.w_bytes = n64 * kp;
-    hipLaunchKernelGGL((int8_group_kernel<T>), dim3((unsigned)((a.tokens + kGroup - 1) / kGroup)), dim3(256), (unsigned)(kp * kGroup), s, g, a.x, a.x_row, a.k);
+    for (int64_t t0 = 0; t0 < a.tokens; t0 += kGroupMost) {
+      g.tokens = std::min(kGroupMost, a.tokens - t0);
+      g.out = (char*)a.out + t0 * a.out_row * kElem<T>;
+      hipLaunchKernelGGL((int8_group_kernel<T>), dim3((unsigned)((g.tokens + kGroup - 1) / kGroup)), dim3(256), (unsigned)(kp * kGroup), s, g,
+                         (const char*)a.x + t0 * a.x_row * kElem<T>, a.x_row, a.k);
+    }
     return;
   }
   // The weights as panels where many token tiles read them, and where 16-byte
