@@ -343,7 +343,8 @@ __global__ __launch_bounds__(256) void fragments_kernel(const int8_t* __restrict
   *(unsigned*)(out + (int64_t)(c >> 5) * kp * 32 + (k0 >> 5) * 1024 + ((k0 >> 4) & 1) * 512 + (c & 31) * 16 + (k0 & 15)) = v;
 }
 
-template <int T>
+// kFar: output rows more than 2^22 elements apart, stored at 64-bit addresses.
+template <int T, bool kFar>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void int8_group_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {
 #ifdef __HIP_DEVICE_COMPILE__
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int c = tile * 64 + y * 32 + l31;
       const bool in = c < g.n;
       const float sw = scales[y], b = g.bias ? biases[y] : 0.f;
-      const int vout = in ? (4 * h * (int)g.out_row + c) * kOut : -1;
+      const int vout = kFar ? 0 : in ? (4 * h * (int)g.out_row + c) * kOut : -1;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -479,6 +480,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float v = (float)acc[i][y][4 * q + e] * se[e] * sw + b;
+            if constexpr (kFar) {
+              if (in && r + 4 * h + e < trows) op_store<T>(g.out, (t0 + r + 4 * h + e) * g.out_row + c, v);
+              continue;
+            }
             const int so = (r + e) * (int)g.out_row * kOut;
             if constexpr (T == kOpF32) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), ro, vout, so, 0);
             else if constexpr (T == kOpBF16) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), ro, vout, so, 0);
@@ -780,6 +785,12 @@ bool mid(int64_t tokens, int64_t k, int64_t n) {
   return !fused(tokens, k) && k <= 1536 && (tokens + 15) / 16 * ((n + 63) / 64) <= 512;
 }
 
+// Many tokens, two workgroups' integers in a CU's LDS (K up to 1216), weights at
+// 32-bit offsets.
+bool group(int64_t tokens, int64_t k, int64_t n) {
+  return tokens >= kGroupTokens && pad64(k) * kGroup <= kGroupLds && pad64(n) * pad64(k) < 0x40000000;
+}
+
 // Tokens of one quantise + multiply round: their integers stay below 1 GiB, which
 // 32-bit offsets reach.
 int64_t round_tokens(int64_t tokens, int64_t k) { return std::min(tokens, std::max<int64_t>(256, ((int64_t)1 << 30) / pad64(k) / 256 * 256)); }
@@ -815,17 +826,19 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
     }
     return;
   }
-  // Many tokens, two workgroups' integers in a CU's LDS (K up to 1216), 32-bit offsets.
-  const int64_t n64 = pad64(a.n);
-  if (a.tokens >= kGroupTokens && kp * kGroup <= kGroupLds && n64 * kp < 0x40000000 && a.out_row <= 1 << 22) {
-    hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, wp);
-    g.w = wp;
+  if (group(a.tokens, a.k, a.n)) {  // the workspace holds the weights alone
+    const int64_t n64 = pad64(a.n);
+    int8_t* fragments = (int8_t*)workspace;
+    hipLaunchKernelGGL(fragments_kernel, dim3((unsigned)(n64 / 16), (unsigned)(kp / 64)), dim3(256), 0, s, a.w, a.w_row, a.n, a.k, (int)kp, fragments);
+    g.w = fragments;
     g.w_bytes = n64 * kp;
     for (int64_t t0 = 0; t0 < a.tokens; t0 += kGroupMost) {
       g.tokens = std::min(kGroupMost, a.tokens - t0);
       g.out = (char*)a.out + t0 * a.out_row * kElem<T>;
-      hipLaunchKernelGGL((int8_group_kernel<T>), dim3((unsigned)((g.tokens + kGroup - 1) / kGroup)), dim3(256), (unsigned)(kp * kGroup), s, g,
-                         (const char*)a.x + t0 * a.x_row * kElem<T>, a.x_row, a.k);
+      const dim3 grid((unsigned)((g.tokens + kGroup - 1) / kGroup));
+      const void* x = (const char*)a.x + t0 * a.x_row * kElem<T>;
+      if (a.out_row <= 1 << 22) hipLaunchKernelGGL((int8_group_kernel<T, false>), grid, dim3(256), (unsigned)(kp * kGroup), s, g, x, a.x_row, a.k);
+      else hipLaunchKernelGGL((int8_group_kernel<T, true>), grid, dim3(256), (unsigned)(kp * kGroup), s, g, x, a.x_row, a.k);
     }
     return;
   }
@@ -859,6 +872,7 @@ void launch_int8_t(Int8Args a, void* workspace, hipStream_t s) {
 int64_t int8_workspace(int64_t tokens, int64_t k, int64_t n) {
   if (tokens <= 0 || k <= 0 || n <= 0) return 0;
   if (fused(tokens, k) || mid(tokens, k, n)) return 0;
+  if (group(tokens, k, n)) return pad256(pad64(n) * pad64(k));
   const int64_t most = round_tokens(tokens, k);
   return pad256(most * 4) + pad256(most * pad64(k)) + pad256(pad64(n) * pad64(k));
 }
