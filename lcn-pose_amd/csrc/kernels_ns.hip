@@ -911,14 +911,16 @@ void launch_thin(const NsArgs& a, void* workspace, hipStream_t s) {
     hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kSolo>), dim3(1, (unsigned)a.batch), dim3(G::kThreads), G::kLds, s, a, p, 0, part, ws, 0);
     return;
   }
-  const dim3 grid(p.slabs, (unsigned)a.batch);
-  const int parts = norm_parts(a);
-  launch_norm<T, kMuon>(a, parts, part, s);
-  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kFirst>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, 1);
-  int set = 0;
-  for (int k = 0; k + 1 < a.steps; ++k, set ^= 1)
-    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kMid>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
-  hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kLast>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
+  if constexpr (G::W > 64) {  // (of 64 columns at most there is one chunk)
+    const dim3 grid(p.slabs, (unsigned)a.batch);
+    const int parts = norm_parts(a);
+    launch_norm<T, kMuon>(a, parts, part, s);
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kFirst>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, 1);
+    int set = 0;
+    for (int k = 0; k + 1 < a.steps; ++k, set ^= 1)
+      hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kMid>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
+    hipLaunchKernelGGL((ns_thin_kernel<MB, WB, NW, T, kMuon, kLast>), grid, dim3(G::kThreads), G::kLds, s, a, p, parts, part, ws, set);
+  }
 }
 
 // The path of a matrix by its sides: short side at most 64 in one launch where the
