@@ -309,9 +309,11 @@ int lcn_muon_update(int32_t device, void* stream, int32_t grad_dtype, int64_t ba
 /* Product in 8-bit integers with one scale a token and one a channel:
  *   s[t] = max_k |x[t,k]| / 127,  q[t,k] = rint(x[t,k] * (127 / max_k |x[t,k]|))
  *   out[t,c] = (sum_k q[t,k] weight[c,k]) * s[t] * weight_scale[c] (+ bias[c])
- * x [tokens][k] and out [tokens][n] of type dtype, weight [n][k] int8, scales
- * and bias float32.  A row of x whose largest magnitude is below 2^-100 counts
- * as zero; one that holds an infinity or a NaN gives NaN.  k <= 131072. */
+ * (the factors of out in this order, in float32: their partial product must stay
+ * inside its range).  x [tokens][k] and out [tokens][n] of type dtype, weight
+ * [n][k] int8, scales and bias float32.  A row of x whose largest magnitude is
+ * below 2^-100 counts as zero; one that holds an infinity or a NaN gives NaN.
+ * k <= 131072, tokens <= 2^30. */
 int64_t lcn_int8_linear_workspace(int64_t tokens, int64_t k, int64_t n);
 int lcn_int8_linear(int32_t device, void* stream, int32_t dtype, int64_t tokens, int64_t k, int64_t n,
                     const void* x, int64_t x_row, const int8_t* weight, int64_t weight_row,

@@ -630,7 +630,8 @@ __global__ __launch_bounds__(256) void int8_few_kernel(Int8Gemm g, const void* _
 // the 16 tokens by 16 channels over every fourth 64-byte piece of K, whose weights
 // are asked for before the quantisation starts; the four sums of a block meet in
 // LDS.  One launch, no workspace.  Bound by latency (the rows, their largest
-// magnitude, the weights): 200 x 1088 x 1088 in 6.3 us, 8.8 with 4 waves, 6.9 with 8.
+// magnitude, the weights): 200 x 1088 x 1088 in 6.3 us a launch of a graph (5.8 us the
+// kernel itself), 8.8 with 4 waves, 6.9 with 8.
 constexpr int kMidWaves = 16;
 template <int T>
 __global__ __launch_bounds__(64 * kMidWaves) __attribute__((amdgpu_waves_per_eu(8))) void int8_mid_kernel(Int8Gemm g, const void* __restrict__ x, int64_t x_row, int k) {

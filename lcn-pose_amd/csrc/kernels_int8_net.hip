@@ -9,7 +9,8 @@
 // where the layer's input is a z), the result is written to them with the BN
 // statistics of the fp32 GEMM's epilogue; absent blocks are skipped as there.
 // Bound by memory: a layer of 65 536 poses x 1088 reads 285 MB of activations and
-// writes 71 MB of integers, then reads those and writes 285 MB of z.
+// writes 71 MB of integers (66 us, 72 with BatchNorm: 5.0 to 5.4 TB/s), then reads those
+// and writes 285 MB of z (128 us, 2.8 TB/s).  The weights of six layers take 15 us.
 #include "gemm_epilogue.h"
 #include "ops_common.h"
 

@@ -947,6 +947,11 @@ int path_of(int64_t rows, int64_t cols) {
 // 1000 (432 / 864 / 1632) 939 / 980 / 1020 (4352 on another card 4750 / 4965).  The
 // update X <- B X, 128 x 128 / 64 x 64: six 1088 (486 / 1734) 54 / 62 us, one (81 /
 // 289) 26 / 16, one 2000 54 / 76.
+// The rules compare rounds (256 tiles each) times what a round of a tile size takes.
+// The times of a round are fitted to these measurements, in units of their own:
+// symmetric products, 128 x 64 : 128 x 128 as 13 : 21, a single round of the latter 27
+// (nothing runs under its first loads and last stores); the update, 64 x 64 : 128 x
+// 128 as 13 : 40 (8.9 : 27 us for six 1088).
 template <int MODE, int T>
 void launch_prod(NsProd g, const NsArgs& a, const NsPlan& p, hipStream_t s) {
   constexpr bool kSym = MODE == kGram || MODE == kSquare;
