@@ -285,9 +285,10 @@ int lcn_eval_mpjpe_static(int32_t device, int64_t n, const double* pred, const d
  *   X = G / max(|G|_F, eps);  steps times: A = X X^T, X <- a X + (b A + c A A) X
  * (on the transpose where rows > cols), (a, b, c) = coefficients[0..2].
  * Muon's are 3.4445, -4.775, 2.0315 with 5 steps.  Products are accurate to
- * float32, measured on a matrix's norm, for every dtype.  The polynomial must keep the singular values of X
- * below 2 and b A + c A A below 16 (beyond: infinities; Muon's stays below 1.3
- * and 7).  A matrix that holds an infinity or a NaN gives NaN.  out may be `in` itself. */
+ * float32, measured on a matrix's norm, for every dtype.  The polynomial must
+ * keep the singular values of X below 2 and a I + b A + c A A below 16 (beyond:
+ * infinities; Muon's stay below 1.3 and 4).  A matrix that holds an infinity or
+ * a NaN gives NaN.  out may be `in` itself. */
 int64_t lcn_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
 int lcn_orthogonalize(int32_t device, void* stream, int32_t dtype, int64_t batch, int64_t rows, int64_t cols,
                       const void* in, int64_t in_batch, int64_t in_row, void* out, int64_t out_batch,
